@@ -324,6 +324,13 @@ thread_local const cudaAccessPolicyWindow* t_l2_window = nullptr;
 const cudaAccessPolicyWindow* current_l2_window() { return t_l2_window; }
 void set_current_l2_window(const cudaAccessPolicyWindow* w) { t_l2_window = w; }
 int internal_fail(int code, const std::string& msg) { return fail(code, msg); }
+int unit_device(int* device, int* num_sms) {
+  BBH_CUDA(cudaGetDevice(device));
+  const int rc = check_sm100(*device);
+  if (rc) return rc;
+  *num_sms = g_num_sms(*device);
+  return BBH_OK;
+}
 void ws_limits(const bbh_ws* ws, int* device, int* max_tokens, int* max_batch, int* max_len) {
   *device = ws->device;
   *max_tokens = ws->max_tokens;

@@ -347,16 +347,21 @@ static PFN_encodeTiled get_encode_fn() {
 // sw128_kmajor_desc; outputs: 32 x 32, 64-byte swizzle, matching ChunkStore).
 int encode_2d(CUtensorMap* map, const __half* base, int rows, int cols, int ld, int box_cols, int box_rows,
               CUtensorMapSwizzle swz) {
+  return encode_2d_bytes(map, base, rows, cols, ld, 2, box_cols, box_rows, swz);
+}
+
+int encode_2d_bytes(CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int elem_bytes, int box_cols,
+                    int box_rows, CUtensorMapSwizzle swz) {
   PFN_encodeTiled enc = get_encode_fn();
   if (!enc) return BBH_ERR_CUDA;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || (ld * 2) % 16) return BBH_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (ld * elem_bytes) % 16) return BBH_ERR_ARG;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * elem_bytes};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUtensorMapDataType type = elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? BBH_OK : BBH_ERR_CUDA;
 }
 

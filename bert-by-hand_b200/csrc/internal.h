@@ -52,6 +52,19 @@ cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sm
 // ------------------------------------------------------------------ C ABI internals
 // Sets the calling thread's bbh_last_error() message and returns code.
 int internal_fail(int code, const std::string& msg);
+// The calling thread's current device, which has to be an sm_100, and its SM count.
+int unit_device(int* device, int* num_sms);
+// Rows [rows, cols] of `bytes`-wide elements, `ld` elements apart: the first byte, the one
+// behind the last, and the stride; for refusing outputs that overlap inputs. rows >= 1.
+struct Span {
+  uintptr_t lo, hi;
+  int64_t ld;
+};
+inline Span span(const void* p, int64_t ld, int rows, int cols, int bytes) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+  return {lo, lo + (uintptr_t(rows - 1) * uintptr_t(ld) + uintptr_t(cols)) * uintptr_t(bytes), ld};
+}
+inline bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
 // Device and capacity of a workspace.
 void ws_limits(const bbh_ws* ws, int* device, int* max_tokens, int* max_batch, int* max_len);
 // The workspace's slot for the corpus driver's staging state; free_fn releases it when
@@ -111,6 +124,9 @@ int make_gemm_plan(GemmPlan* plan, const __half* A, int lda, int rows_cap, const
 // box_cols x box_rows with the given swizzle. Returns 0 or a BBH_ERR_*.
 int encode_2d(CUtensorMap* map, const __half* base, int rows, int cols, int ld, int box_cols, int box_rows,
               CUtensorMapSwizzle swz);
+// The same for elements of 1 byte or of 2 (any 16-bit type), int64 row stride.
+int encode_2d_bytes(CUtensorMap* map, const void* base, int rows, int cols, int64_t ld, int elem_bytes, int box_cols,
+                    int box_rows, CUtensorMapSwizzle swz);
 // kEpiResLN: the residual [rows_cap, N] with row stride ldr (read with TMA, 16-byte aligned).
 int set_gemm_residual(GemmPlan* plan, const __half* R, int ldr);
 cudaError_t launch_gemm(const GemmPlan& plan, cudaStream_t stream, bool pdl = false);

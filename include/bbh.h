@@ -186,6 +186,53 @@ BBH_API int bbh_attention_varlen(const uint16_t* qkv, uint16_t* ctx, const int32
 BBH_API int bbh_mean_pool_l2(const uint16_t* hidden, const int32_t* cu_seqlens, const uint8_t* tokmask, int batch,
                      uint16_t* emb, void* stream);
 
+/* ---- unit operators of the 8-bit linear path -----------------------------------------
+ * No counterpart in the reference (fp16 only). A linear layer on int8 operands with one fp32
+ * scale per token and per output channel, and the row operators that make its operands. A
+ * "row" is a token or an output channel; value (i, d) of 8-bit rows stands for
+ * q[i, d] * scale[i]. Row strides (ld*, in elements) may exceed the row length; other bytes
+ * between rows are neither read nor written. 16-bit tensors are fp16 or bf16 by `dtype`, all
+ * of one call the same; every product and sum is fp32 (linear_i8: int32) and each output is
+ * rounded once. M = 0 does nothing. Outputs must not overlap inputs or one another (the
+ * exceptions are named); the pointers belong to the current device. No workspace, no
+ * allocation, no state between calls: calls may run on any streams at once and be captured
+ * into CUDA graphs. The kernels launch with programmatic dependent launch. */
+#define BBH_F16 0
+#define BBH_BF16 1
+#define BBH_ROW_MAX_D 32768
+#define BBH_LINEAR_I8_MAX_K 131071
+/* v = x + residual (fp32, not rounded; residual may be NULL); y = v / sqrt(mean(v^2) + eps) *
+ * weight (NULL: ones). sum (NULL, or with a residual) receives v rounded to dtype. y and sum
+ * may each be x or residual itself (same pointer, same stride). D in [1, 32768]. */
+BBH_API int bbh_rmsnorm(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr, const uint16_t* weight,
+                        uint16_t* y, int64_t ldy, uint16_t* sum, int64_t lds, int M, int D, float eps, int dtype,
+                        void* stream);
+/* The same norm with y left in 8 bits: scale[i] = max_d |y[i, d]| / 127, q = y / scale[i]
+ * rounded half to even, from y unrounded. A row whose largest |v * weight| is below 2^-120 gets
+ * scale 0 and zeros; a row with a NaN or an infinity gets scale NaN and zeros, so that every
+ * result computed from it is NaN. sum may be x or residual itself. */
+BBH_API int bbh_rmsnorm_i8(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr,
+                           const uint16_t* weight, int8_t* q, int64_t ldq, float* scale, uint16_t* sum, int64_t lds,
+                           int M, int D, float eps, int dtype, void* stream);
+/* Rows of x [M, D] to 8 bits as above (y = x): activations of any origin with one scale per
+ * token, or nn.Linear weights [N, K] with one scale per output channel. */
+BBH_API int bbh_quantize_i8(const uint16_t* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int M, int D,
+                            int dtype, void* stream);
+/* y = q * scale[row], rounded to dtype. */
+BBH_API int bbh_dequantize_i8(const int8_t* q, int64_t ldq, const float* scale, uint16_t* y, int64_t ldy, int M, int D,
+                              int dtype, void* stream);
+/* C[M, N] = (A W^T) * a_scale[m] * w_scale[n] (+ bias[n]) (+ erf-GELU as bbh_linear's), A [M, K]
+ * and W [N, K] (nn.Linear layout) int8, exact int32 sums. A and W 16-byte aligned with row
+ * strides of whole 16 bytes (K itself may be any value in [1, 131071]); C and bias (dtype, bias
+ * may be NULL) of any alignment and N. */
+BBH_API int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw,
+                          const float* w_scale, const uint16_t* bias, uint16_t* C, int64_t ldc, int M, int N, int K,
+                          int gelu, int dtype, void* stream);
+/* Synchronises the current device and returns the device error code of its bbh_linear_i8 calls
+ * (0 = none, 1 = a wait inside a kernel ran out: that call's output is invalid); optionally
+ * clears it. */
+BBH_API int bbh_linear_i8_device_error(int reset);
+
 /* ---- host corpus driver --------------------------------------------------------------
  * The reference's corpus loop (bench/corpus.cu:80-160) as a library call: sort the
  * sentences by length, cut batches, run them, gather the embeddings back to corpus order.
