@@ -63,28 +63,39 @@ __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
 constexpr int kBK = 128;  // int8 per k-block: one 128-byte swizzle row
 constexpr int kMmaK = 32;
 
-// erf-GELU of the layer's output. fp16: gelu_half2, the one of bbh_linear. bf16: the same fit,
-//   y(x) = x p(x^2), gelu = x/2 (1 + tanh y), evaluated in fp32 (no clamp: p > 0 everywhere).
-__device__ __forceinline__ float gelu_f32(float x) {
-  const float u = x * x;
-  float z = fmaf(1.19315286e-06f, u, -3.22934132e-05f);
-  z = fmaf(z, u, -1.12335663e-04f);
-  z = fmaf(z, u, 3.64356497e-02f);
-  z = fmaf(z, u, 7.97853484e-01f);
-  float t;
-  asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(z * x));
-  return fmaf(0.5f * x, t, 0.5f * x);
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// Two outputs rounded to 16 bits, packed (a in the low half).
+// erf-GELU, x Phi(x) = max(x, 0) - |x| Phi(-|x|), on a pair of fp32 values (packed f32x2 fmas).
+// log2 Phi(-a) is close to a parabola and is evaluated as a polynomial of degree 10 in a (this
+// project's own least-squares fit on [0, 5.75], reweighted to equal ripple; relative error of
+// Phi at most 2.2e-6, 3.3e-7 rms); beyond 5.75 the polynomial keeps falling, and Phi with it, so no
+// clamp is needed. |error| < 1e-6 max(|x|, 1) with ex2.approx's 2^-22.
+__device__ __forceinline__ unsigned long long gelu2(unsigned long long x) {
+  constexpr float kPhi[11] = {-0.99999976158f,    -1.1511156559f,     -0.4591409266f,    -0.0526544638f,
+                              0.00723045366f,     -0.00021254165f,    -0.000184435105f,  5.04806158e-05f,
+                              -6.74621288e-06f,   4.83748636e-07f,    -1.48185313e-08f};
+  const unsigned long long a = x & 0x7fffffff7fffffffull;
+  unsigned long long p = f2(kPhi[10], kPhi[10]);
+#pragma unroll
+  for (int i = 9; i >= 0; --i) p = f2_fma(p, a, f2(kPhi[i], kPhi[i]));
+  const float2 e = f2_split(p), xs = f2_split(x);
+  const unsigned long long phi = f2(ex2(e.x), ex2(e.y));
+  return f2_fma(a ^ 0x8000000080000000ull, phi, f2(fmaxf(xs.x, 0.f), fmaxf(xs.y, 0.f)));
+}
+
+// Two outputs (with GELU) rounded to 16 bits, packed (the low half first).
 template <bool BF16, bool GELU>
-__device__ __forceinline__ uint32_t finish2(float a, float b) {
+__device__ __forceinline__ uint32_t finish2(unsigned long long y) {
+  const float2 v = f2_split(GELU ? gelu2(y) : y);
   if constexpr (BF16) {
-    const __nv_bfloat162 h = GELU ? __floats2bfloat162_rn(gelu_f32(a), gelu_f32(b)) : __floats2bfloat162_rn(a, b);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  const uint32_t w = pack_half2(a, b);
-  return GELU ? gelu_half2(w) : w;
+  return pack_half2(v.x, v.y);
 }
 
 template <bool BF16>
@@ -93,9 +104,33 @@ __device__ __forceinline__ float bias_f32(const uint16_t* b) {
   return __half2float(*reinterpret_cast<const __half*>(b));
 }
 
-// (acc * a_scale) * w_scale + bias, the same in both kernels (bit for bit)
-__device__ __forceinline__ float dequant(int acc, float sa, float sw, float bias) {
-  return fmaf(__int2float_rn(acc) * sa, sw, bias);
+// (acc * a_scale) * w_scale + bias of two outputs, the same in both kernels (bit for bit)
+__device__ __forceinline__ unsigned long long dequant2(int acc0, int acc1, unsigned long long sa,
+                                                       unsigned long long sw, unsigned long long bias) {
+  return f2_fma(f2_mul(f2(__int2float_rn(acc0), __int2float_rn(acc1)), sa), sw, bias);
+}
+
+// 32 lanes x 32 columns of TMEM, the load only; tmem_wait32 makes the registers valid.
+__device__ __forceinline__ void tmem_issue32(uint32_t taddr, int (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait32(int (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
 }
 
 // ====================================================================== many rows: SM pairs
@@ -256,75 +291,98 @@ __global__ void __launch_bounds__(I8PairCfg<BN>::THREADS, 1)
     const int part = (warp - 2) >> 2;  // which 64 columns of the tile
     const int we = warp - 2;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-    ChunkStore cst{s_stage + we * 4096, &tmC, lane};
-    float* s_sw = s_cols + we * 128;  // this warp's 64 channel scales, then 64 biases
+    uint8_t* buf = s_stage + we * 4096;  // 32 rows x 64 columns, 16-byte piece c of row r at piece c ^ (r & 7)
+    float* s_sw = s_cols + we * 128;     // this warp's 64 channel scales, then 64 biases
     float* s_b = s_sw + 64;
     const uint32_t acce0 = mapa_shared(smem_u32(acce_bar), 0);
+    // The scales and biases of a tile are fetched while the previous tile is worked on (lane l:
+    // row l, columns l and 32 + l).
+    float sa_next = 0.f, sw_next[2] = {0.f, 0.f}, b_next[2] = {0.f, 0.f};
+    auto fetch = [&](int t) {
+      const int row = tile_m0(t) + quad * 32 + lane;
+      sa_next = row < p.M ? __ldg(p.a_scale + row) : 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = tile_n0(t) + part * 64 + 32 * h + lane;
+        sw_next[h] = c < p.N ? __ldg(p.w_scale + c) : 0.f;
+        b_next[h] = p.bias && c < p.N ? bias_f32<BF16>(p.bias + c) : 0.f;
+      }
+    };
+    if (first_tile < num_tiles) fetch(first_tile);
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
       const int row0 = tile_m0(tile) + quad * 32;
       const int c0 = tile_n0(tile) + part * 64;
-      // this tile's scales, fetched while the MMAs run
-      const float sa = row0 + lane < p.M ? __ldg(p.a_scale + row0 + lane) : 0.f;
-      __syncwarp();  // the previous tile's reads of s_sw / s_b are done
+      if (TMA_C && lane == 0) bulk_wait_read<0>();  // the previous tile's store has read the buffer
+      __syncwarp();  // and its scales and biases have been read by every lane
+      const unsigned long long sa = f2(sa_next, sa_next);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int c = c0 + 32 * h + lane;
-        s_sw[32 * h + lane] = c < p.N ? __ldg(p.w_scale + c) : 0.f;
-        s_b[32 * h + lane] = p.bias && c < p.N ? bias_f32<BF16>(p.bias + c) : 0.f;
+        s_sw[32 * h + lane] = sw_next[h];
+        s_b[32 * h + lane] = b_next[h];
       }
       __syncwarp();
+      if (tile + tile_step < num_tiles) fetch(tile + tile_step);
       if (!mbar_wait(&accf_bar[acc], acc_phase, abort_flag, &g_i8_err)) break;
       tc_fence_after();
       const uint32_t tacc = tmem_base + lane_off + acc * BN + part * 64;
-      float v[64];  // int32 accumulators
-      tmem_ld64(tacc, tacc + 32, v);
-      // accumulator read: release it to the even CTA's MMA thread
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acce0 + acc * 8);
-      uint32_t w[32];
+      int v[2][32];
+      tmem_issue32(tacc, v[0]);
+      tmem_wait32(v[0]);
+      tmem_issue32(tacc + 32, v[1]);  // arrives while the first half is worked on
+      uint8_t* rowp = buf + lane * 128;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float4 sw = *reinterpret_cast<const float4*>(s_sw + 4 * j);
-        const float4 b = *reinterpret_cast<const float4*>(s_b + 4 * j);
-        const float y0 = dequant(__float_as_int(v[4 * j]), sa, sw.x, b.x);
-        const float y1 = dequant(__float_as_int(v[4 * j + 1]), sa, sw.y, b.y);
-        const float y2 = dequant(__float_as_int(v[4 * j + 2]), sa, sw.z, b.z);
-        const float y3 = dequant(__float_as_int(v[4 * j + 3]), sa, sw.w, b.w);
-        w[2 * j] = finish2<BF16, GELU>(y0, y1);
-        w[2 * j + 1] = finish2<BF16, GELU>(y2, y3);
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1) {
+          tmem_wait32(v[1]);
+          // accumulator read: release it to the even CTA's MMA thread
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acce0 + acc * 8);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int k = 8 * c + 4 * j;
+            const ulonglong2 sw = *reinterpret_cast<const ulonglong2*>(s_sw + 32 * h + k);
+            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + 32 * h + k);
+            w[2 * j] = finish2<BF16, GELU>(dequant2(v[h][k], v[h][k + 1], sa, sw.x, b.x));
+            w[2 * j + 1] = finish2<BF16, GELU>(dequant2(v[h][k + 2], v[h][k + 3], sa, sw.y, b.y));
+          }
+          *reinterpret_cast<uint4*>(rowp + (((4 * h + c) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
       if constexpr (TMA_C) {
-        if (c0 < p.N && row0 < p.M) cst.put64(w, c0, row0);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0 && c0 < p.N && row0 < p.M) {
+          tma_store_2d(&tmC, buf, c0, row0);
+          bulk_commit();
+        }
       } else {
-        // 32 rows x 64 columns through the staging buffer (16-byte piece c of row r at piece
-        // c ^ (r & 7)), then row by row: 32 neighbouring 2-byte stores at a time
-        uint8_t* rowp = cst.buf + lane * 128;
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(rowp + ((c ^ (lane & 7)) << 4)) =
-              make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        // row by row: 32 neighbouring 2-byte stores at a time
         __syncwarp();
         const int rows = min(32, p.M - row0);
         for (int r = 0; r < rows; ++r) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int col = 32 * h + lane;
-            const uint16_t o = *reinterpret_cast<const uint16_t*>(cst.buf + r * 128 + (((col >> 3) ^ (r & 7)) << 4) +
-                                                                  (col & 7) * 2);
+            const uint16_t o =
+                *reinterpret_cast<const uint16_t*>(buf + r * 128 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2);
             if (c0 + col < p.N) p.C[static_cast<int64_t>(row0 + r) * p.ldc + c0 + col] = o;
           }
         }
-        __syncwarp();
       }
       if (++acc == NACC) {
         acc = 0;
         acc_phase ^= 1;
       }
     }
-    if (TMA_C) cst.drain();
+    if (TMA_C && lane == 0) bulk_wait_all();
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -351,43 +409,52 @@ struct I8SmallCfg {
   static constexpr int A_BYTES = 128 * kBK;  // 128 output channels of W
   static constexpr int B_BYTES = BN * kBK;   // BN tokens
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int RED_BYTES = BN * 512;  // partial sums of this CTA's tokens from every CTA of the cluster
+  // partial sums of the tokens that a CTA finishes, from every CTA of the cluster: int32
+  // [splits][128 channels][tokens], at least 4 tokens a CTA, at most 8 CTAs
+  static constexpr int RED_BYTES = (BN < 32 ? 32 : BN) * 512;
   static constexpr int STAGES = (204 * 1024 - RED_BYTES) / STAGE_BYTES > 8 ? 8 : (204 * 1024 - RED_BYTES) / STAGE_BYTES;
   static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
-  static constexpr int THREADS = 64 + 128;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + RED_BYTES + 1024 + 256;
+  static constexpr int PARTS = BN < 64 ? 1 : 2;  // epilogue warps per TMEM lane quadrant, BN / PARTS tokens each
+  static constexpr int THREADS = 64 + 128 * PARTS;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + RED_BYTES + 1024 + 256 + 4 * BN;
   static_assert((BN & (BN - 1)) == 0 && BN >= 16 && BN <= 128, "token tile");
-  // One CTA per SM (so TMEM, 128 columns at most, can always be had), see launch_small.
+  // more than half an SM's shared memory: one CTA per SM, so TMEM can always be had
   static_assert(SMEM > 114 * 1024 && SMEM <= 227 * 1024, "shared memory");
 };
 
-// grid: x = cluster size * channel tiles, y = token tiles; rank r of a cluster sums the r-th part
-// of the k-blocks and finishes the tokens t = r (mod cluster size) of the tile.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// grid: x = cluster size (2^log_splits) * channel tiles, y = token tiles. Rank r of a cluster sums the
+// r-th part of the k-blocks and finishes the r-th `per` tokens of the tile.
 template <int BN, bool BF16, bool GELU>
 __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
     linear_i8_small_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                           const I8Params p, const int splits) {
+                           const I8Params p, const int log_splits) {
   using Cfg = I8SmallCfg<BN>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * Cfg::A_BYTES;
-  int* red = reinterpret_cast<int*>(smem + STAGES * Cfg::STAGE_BYTES);  // [splits][BN / splits][128]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::RED_BYTES);
+  uint8_t* red = smem + STAGES * Cfg::STAGE_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(red + Cfg::RED_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* acc_bar = empty_bar + STAGES;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(acc_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  float* s_sa = reinterpret_cast<float*>(red + Cfg::RED_BYTES + 256);  // [BN] token scales
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int n0 = static_cast<int>(blockIdx.x) / splits * 128;
+  const int splits = 1 << log_splits;
+  const int rank = log_splits ? static_cast<int>(cluster_ctarank()) : 0;
+  const int n0 = (static_cast<int>(blockIdx.x) >> log_splits) * 128;
   const int m0 = static_cast<int>(blockIdx.y) * BN;
   const int k_blocks = (p.K + kBK - 1) / kBK;
-  const int kb0 = static_cast<int>(static_cast<int64_t>(k_blocks) * rank / splits);
-  const int kb1 = static_cast<int>(static_cast<int64_t>(k_blocks) * (rank + 1) / splits);
+  const int kb0 = (k_blocks * rank) >> log_splits;
+  const int kb1 = (k_blocks * (rank + 1)) >> log_splits;
+  const int tokens = min(BN, p.M - m0);
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -402,13 +469,12 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
     tma_prefetch_desc(&tmX);
   }
   if (warp == 1) tmem_alloc(tmem_holder, Cfg::TMEM_COLS);
-  pdl_wait();
   tc_fence_before();
   __syncthreads();
-  if (splits > 1) cluster_sync_all();  // every CTA of the cluster runs: its shared memory may be written
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  const int tokens = min(BN, p.M - m0);
+  pdl_wait();
+  if (log_splits) cluster_arrive();  // this CTA runs: its shared memory may be written (waited for below)
 
   if (warp == 0) {
     if (lane == 0) {
@@ -455,71 +521,93 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
     __syncwarp();
   }
 
-  // Epilogue threads: lane of TMEM = output channel, column = token.
+  // Epilogue threads: TMEM lane = output channel, column = token. Each thread has one channel and
+  // works on groups of four tokens.
+  const bool epi = warp >= 2;
   const int quad = warp & 3;
+  const int part = epi ? (warp - 2) >> 2 : 0;
   const int ch = quad * 32 + lane;
   const int n = n0 + ch;
-  const bool epi = warp >= 2;
-  bool ok = false;
-  float sw = 0.f, bias = 0.f;
-  if (epi) {
+  unsigned long long sw = 0, bias = 0;
+  auto put4 = [&](int t, int4 a) {
+    const ulonglong2 sa = *reinterpret_cast<const ulonglong2*>(s_sa + t);
+    const uint32_t w0 = finish2<BF16, GELU>(dequant2(a.x, a.y, sa.x, sw, bias));
+    const uint32_t w1 = finish2<BF16, GELU>(dequant2(a.z, a.w, sa.y, sw, bias));
     if (n < p.N) {
-      sw = __ldg(p.w_scale + n);
-      bias = p.bias ? bias_f32<BF16>(p.bias + n) : 0.f;
-    }
-    ok = mbar_wait(acc_bar, 0, abort_flag, &g_i8_err);
-    __syncwarp();
-    tc_fence_after();
-  }
-  // two tokens of one channel: 2-byte stores, 32 neighbouring channels per warp
-  auto put = [&](int t, int a0, int a1) {
-    const float s0 = __ldg(p.a_scale + m0 + t);
-    const bool two = t + splits < tokens;
-    const float s1 = two ? __ldg(p.a_scale + m0 + t + splits) : 0.f;
-    const uint32_t w = finish2<BF16, GELU>(dequant(a0, s0, sw, bias), dequant(a1, s1, sw, bias));
-    uint16_t* c = p.C + static_cast<int64_t>(m0 + t) * p.ldc + n;
-    if (n < p.N) {
-      c[0] = static_cast<uint16_t>(w);
-      if (two) c[splits * p.ldc] = static_cast<uint16_t>(w >> 16);
+      uint16_t* c = p.C + static_cast<int64_t>(m0 + t) * p.ldc + n;
+      c[0] = static_cast<uint16_t>(w0);
+      if (t + 1 < tokens) c[p.ldc] = static_cast<uint16_t>(w0 >> 16);
+      if (t + 2 < tokens) c[2 * p.ldc] = static_cast<uint16_t>(w1);
+      if (t + 3 < tokens) c[3 * p.ldc] = static_cast<uint16_t>(w1 >> 16);
     }
   };
-  const uint32_t tacc = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-  const bool all_ok = __all_sync(0xffffffffu, ok);
-  if (epi && all_ok) {
+  // partial sums: int4 g (tokens 4 g ..) of channel ch from rank src at [src][ch][g], the 16-byte pieces of
+  // a channel permuted so that eight neighbouring channels' accesses fall into different banks
+  const int log_per = max(2, (31 - __clz(BN)) - log_splits);  // tokens a CTA finishes: 2^log_per
+  const int pieces = 1 << (log_per - 2);
+  const int swz = pieces >= 8 ? (ch & 7) : ((ch * pieces) >> 3) & (pieces - 1);
+  bool ok = true;
+  if (epi) {
+    const int e = threadIdx.x - 64;
+    if (e < BN) s_sa[e] = e < tokens ? __ldg(p.a_scale + m0 + e) : 0.f;
+    if (n < p.N) {
+      const float s = __ldg(p.w_scale + n);
+      const float b = p.bias ? bias_f32<BF16>(p.bias + n) : 0.f;
+      sw = f2(s, s);
+      bias = f2(b, b);
+    }
+    named_barrier(1, 128 * Cfg::PARTS);  // the token scales are in place
+    ok = mbar_wait(acc_bar, 0, abort_flag, &g_i8_err);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+  }
+  if (log_splits) cluster_wait();  // every CTA of the cluster runs
+  if (epi && ok) {
+    const uint32_t tacc = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const int t_end = min(tokens, (part + 1) * (BN / Cfg::PARTS));
 #pragma unroll 1
-    for (int c = 0; c < tokens; c += 32) {  // BN = 16: the 16 columns behind the tile are not used
-      float v[32];
-      tmem_ld32(tacc + c, v);
-      if (splits == 1) {
+    for (int c = part * (BN / Cfg::PARTS); c < t_end; c += 32) {  // BN = 16: the upper 16 columns are not used
+      int v[32];
+      tmem_issue32(tacc + c, v);
+      tmem_wait32(v);
 #pragma unroll
-        for (int t = 0; t < 32; t += 2)
-          if (c + t < tokens) put(c + t, __float_as_int(v[t]), __float_as_int(v[t + 1]));
-      } else {
-        const uint32_t own = smem_u32(red + (rank * (BN / splits)) * 128 + ch);
-#pragma unroll
-        for (int t = 0; t < 32; ++t)
-          if (c + t < tokens) {
-            const int to = (c + t) & (splits - 1), slot = (c + t) / splits;
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa_shared(own + slot * 512, to)),
-                         "r"(__float_as_int(v[t]))
+      for (int g = 0; g < 8; ++g) {
+        const int t = c + 4 * g;
+        const int4 a = make_int4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        if (t < tokens) {
+          if (log_splits == 0) {
+            put4(t, a);
+          } else {
+            const int piece = (t & ((1 << log_per) - 1)) >> 2;
+            const uint32_t at = smem_u32(red) + (((rank * 128 + ch) << log_per) << 2) + ((piece ^ swz) << 4);
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_shared(at, t >> log_per)),
+                         "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w)
                          : "memory");
           }
+        }
       }
     }
   }
-  if (splits > 1) {
+  if (log_splits) {
     __syncwarp();
-    cluster_sync_all();  // all partial sums are in place
+    cluster_arrive();
+    cluster_wait();  // all partial sums are in place
     if (epi) {
-      const int mine = (tokens - rank + splits - 1) / splits;  // tokens rank, rank + splits, ...
-      for (int s = 0; s < mine; s += 2) {
-        int a0 = 0, a1 = 0;
-        for (int src = 0; src < splits; ++src) {
-          const int* part = red + (src * (BN / splits) + s) * 128 + ch;
-          a0 += part[0];
-          if (s + 1 < mine) a1 += part[128];
+      for (int g = part; g < pieces; g += Cfg::PARTS) {
+        const int t = (rank << log_per) + 4 * g;
+        if (t >= tokens) break;
+        int4 a = make_int4(0, 0, 0, 0);
+#pragma unroll 1
+        for (int src = 0; src < splits; src += 2) {
+          const uint8_t* at = red + (((src * 128 + ch) << log_per) << 2) + ((g ^ swz) << 4);
+          const int4 x = *reinterpret_cast<const int4*>(at);
+          const int4 y = *reinterpret_cast<const int4*>(at + ((128 << log_per) << 2));
+          a.x += x.x + y.x;
+          a.y += x.y + y.y;
+          a.z += x.z + y.z;
+          a.w += x.w + y.w;
         }
-        put(rank + s * splits, a0, a1);
+        put4(t, a);
       }
     }
   }
@@ -607,24 +695,24 @@ cudaError_t launch_pair_bn(const I8Maps& m, const I8Params& p, bool bf16, bool g
 }
 
 template <int BN, bool BF16, bool GELU>
-cudaError_t launch_small_i8(const I8Maps& m, const I8Params& p, int splits, int dev, cudaStream_t s) {
+cudaError_t launch_small_i8(const I8Maps& m, const I8Params& p, int log_splits, int dev, cudaStream_t s) {
   using Cfg = I8SmallCfg<BN>;
   static bool done[64] = {};
   auto kern = linear_i8_small_kernel<BN, BF16, GELU>;
   const cudaError_t e = opt_in(kern, Cfg::SMEM, done, dev);
   if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(splits * ((p.N - 1) / 128 + 1)), static_cast<unsigned>((p.M - 1) / BN + 1));
-  return launch_ex(kern, grid, dim3(Cfg::THREADS), Cfg::SMEM, s, true, splits, m.W, m.A, p, splits);
+  const dim3 grid(static_cast<unsigned>(((p.N - 1) / 128 + 1) << log_splits), static_cast<unsigned>((p.M - 1) / BN + 1));
+  return launch_ex(kern, grid, dim3(Cfg::THREADS), Cfg::SMEM, s, true, 1 << log_splits, m.W, m.A, p, log_splits);
 }
 
 template <int BN>
-cudaError_t launch_small_bn(const I8Maps& m, const I8Params& p, bool bf16, bool gelu, int splits, int dev,
+cudaError_t launch_small_bn(const I8Maps& m, const I8Params& p, bool bf16, bool gelu, int log_splits, int dev,
                             cudaStream_t s) {
   if (bf16)
-    return gelu ? launch_small_i8<BN, true, true>(m, p, splits, dev, s)
-                : launch_small_i8<BN, true, false>(m, p, splits, dev, s);
-  return gelu ? launch_small_i8<BN, false, true>(m, p, splits, dev, s)
-              : launch_small_i8<BN, false, false>(m, p, splits, dev, s);
+    return gelu ? launch_small_i8<BN, true, true>(m, p, log_splits, dev, s)
+                : launch_small_i8<BN, true, false>(m, p, log_splits, dev, s);
+  return gelu ? launch_small_i8<BN, false, true>(m, p, log_splits, dev, s)
+              : launch_small_i8<BN, false, false>(m, p, log_splits, dev, s);
 }
 
 }  // namespace
@@ -670,15 +758,15 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
     const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const int k_blocks = (K + kBK - 1) / kBK;
     const int tiles = ch_tiles * ((M - 1) / bn + 1);
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 <= k_blocks) splits *= 2;
+    int log_splits = 0;
+    while (log_splits < 3 && (tiles << (log_splits + 1)) <= sms && (2 << log_splits) <= k_blocks) ++log_splits;
     rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, bn, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return internal_fail(rc, "bbh_linear_i8: tensor map encoding failed");
-    e = bn == 16   ? launch_small_bn<16>(maps, p, bf16, g, splits, dev, s)
-        : bn == 32 ? launch_small_bn<32>(maps, p, bf16, g, splits, dev, s)
-        : bn == 64 ? launch_small_bn<64>(maps, p, bf16, g, splits, dev, s)
-                   : launch_small_bn<128>(maps, p, bf16, g, splits, dev, s);
+    e = bn == 16   ? launch_small_bn<16>(maps, p, bf16, g, log_splits, dev, s)
+        : bn == 32 ? launch_small_bn<32>(maps, p, bf16, g, log_splits, dev, s)
+        : bn == 64 ? launch_small_bn<64>(maps, p, bf16, g, log_splits, dev, s)
+                   : launch_small_bn<128>(maps, p, bf16, g, log_splits, dev, s);
   } else {
     const int bn = N % 256 && N % 192 == 0 ? 192 : 256;
     rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);

@@ -104,17 +104,23 @@ __device__ __forceinline__ void store8(uint16_t* row, int j, int t, int group, i
   }
 }
 
-// rint(f * inv) as the low byte of f * inv + 1.5 * 2^23: one fma, one rounding (half to even);
-// |f * inv| <= 127 (1 + 2^-23), which rounds to 127 at most.
-__device__ __forceinline__ uint32_t round_byte(float f, float inv) {
+// rint(f * 127 / top) as the low byte of f * inv + 1.5 * 2^23 (rounded half to even there);
+// |f * inv| <= 127 (1 + 2^-23), which rounds to 127 at most. Elements of a 16-bit row meet exact
+// halves (top / 2 is 63.5 steps), which inv = 127 / top rounded to fp32 would push to either
+// side: TIES adds the rest of 127 / top, so that f * 127 / top is right to fp32 and a half
+// stays one (with 11-bit elements every other value is 2^-20 of itself or more away from a half).
+template <bool TIES>
+__device__ __forceinline__ uint32_t round_byte(float f, float inv, float inv_rest) {
+  if constexpr (TIES) return __float_as_uint(fmaf(f, inv, f * inv_rest) + 12582912.f);
   return __float_as_uint(fmaf(f, inv, 12582912.f));
 }
 
-template <int VEC>
-__device__ __forceinline__ void store_q8(int8_t* row, int j, int t, int group, int D, const float* f, float inv) {
+template <int VEC, bool TIES>
+__device__ __forceinline__ void store_q8(int8_t* row, int j, int t, int group, int D, const float* f, float inv,
+                                         float inv_rest) {
   uint32_t b[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) b[i] = inv > 0.f ? round_byte(f[i], inv) : 0u;
+  for (int i = 0; i < 8; ++i) b[i] = inv > 0.f ? round_byte<TIES>(f[i], inv, inv_rest) : 0u;
   if constexpr (VEC == 8) {
     const int e = elem<8>(j, 0, t, group);
     uint2 o;
@@ -235,10 +241,11 @@ __global__ void __launch_bounds__(kRowMaxBlock) row_kernel(const RowParams p) {
     // that whatever is computed from it is NaN too.
     const bool finite = top <= FLT_MAX;
     const float inv = finite && top >= 0x1p-120f ? 127.f / top : 0.f;
+    const float rest = inv > 0.f ? fmaf(-inv, top, 127.f) / top : 0.f;
     if (live && t == 0)
       p.scale[r] = finite ? (inv > 0.f ? top / 127.f : 0.f) * rstd : __int_as_float(0x7fc00000);
 #pragma unroll
-    for (int j = 0; j < V; ++j) store_q8<VEC>(p.q + r * p.ldq, j, t, group, D, f + 8 * j, inv);
+    for (int j = 0; j < V; ++j) store_q8<VEC, MODE == kRowQuant>(p.q + r * p.ldq, j, t, group, D, f + 8 * j, inv, rest);
   }
 }
 
