@@ -54,6 +54,16 @@ __device__ __forceinline__ void tc_mma_i8_pair(uint32_t d_tmem, uint64_t a_desc,
       : "memory");
 }
 
+// Arrive once on the mbarrier at this shared-memory offset in BOTH CTAs of the pair when the pair
+// MMAs issued so far by this thread have finished (one commit: each costs the issuing thread time).
+__device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
 // Instruction descriptor, kind::i8: signed A and B, int32 D, both K-major.
 __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
@@ -69,33 +79,52 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// erf-GELU, x Phi(x) = max(x, 0) - |x| Phi(-|x|), on a pair of fp32 values (packed f32x2 fmas).
-// log2 Phi(-a) is close to a parabola and is evaluated as a polynomial of degree 10 in a (this
-// project's own least-squares fit on [0, 5.75], reweighted to equal ripple; relative error of
-// Phi at most 2.2e-6, 3.3e-7 rms); beyond 5.75 the polynomial keeps falling, and Phi with it, so no
-// clamp is needed. |error| < 1e-6 max(|x|, 1) with ex2.approx's 2^-22.
-__device__ __forceinline__ unsigned long long gelu2(unsigned long long x) {
+// erf-GELU, x Phi(x) = max(x, 0) - |x| Phi(-|x|), of N pairs of fp32 values (packed f32x2 fmas; the
+// pairs go through the polynomial side by side, which hides the fmas' latency and loads each
+// coefficient once). log2 Phi(-a) is close to a parabola and is evaluated as a polynomial of degree 10
+// in a (this project's own least-squares fit on [0, 5.75], reweighted to equal ripple; relative
+// error of Phi at most 2.2e-6, 3.3e-7 rms); beyond 5.75 the polynomial keeps falling, and Phi with it,
+// so no clamp is needed. |error| < 1e-6 max(|x|, 1) with ex2.approx's 2^-22.
+template <int N>
+__device__ __forceinline__ void gelu2(unsigned long long (&x)[N]) {
   constexpr float kPhi[11] = {-0.99999976158f,    -1.1511156559f,     -0.4591409266f,    -0.0526544638f,
                               0.00723045366f,     -0.00021254165f,    -0.000184435105f,  5.04806158e-05f,
                               -6.74621288e-06f,   4.83748636e-07f,    -1.48185313e-08f};
-  const unsigned long long a = x & 0x7fffffff7fffffffull;
-  unsigned long long p = f2(kPhi[10], kPhi[10]);
+  float a[2 * N], p[2 * N];
 #pragma unroll
-  for (int i = 9; i >= 0; --i) p = f2_fma(p, a, f2(kPhi[i], kPhi[i]));
-  const float2 e = f2_split(p), xs = f2_split(x);
-  const unsigned long long phi = f2(ex2(e.x), ex2(e.y));
-  return f2_fma(a ^ 0x8000000080000000ull, phi, f2(fmaxf(xs.x, 0.f), fmaxf(xs.y, 0.f)));
+  for (int q = 0; q < N; ++q) {
+    const float2 r = f2_split(x[q]);
+    a[2 * q] = fabsf(r.x);
+    a[2 * q + 1] = fabsf(r.y);
+    x[q] = f2(fmaxf(r.x, 0.f), fmaxf(r.y, 0.f));
+  }
+#pragma unroll
+  for (int q = 0; q < 2 * N; ++q) p[q] = fmaf(kPhi[10], a[q], kPhi[9]);
+#pragma unroll
+  for (int i = 8; i >= 0; --i)
+#pragma unroll
+    for (int q = 0; q < 2 * N; ++q) p[q] = fmaf(p[q], a[q], kPhi[i]);
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    const float2 r = f2_split(x[q]);
+    x[q] = f2(fmaf(-a[2 * q], ex2(p[2 * q]), r.x), fmaf(-a[2 * q + 1], ex2(p[2 * q + 1]), r.y));
+  }
 }
 
-// Two outputs (with GELU) rounded to 16 bits, packed (the low half first).
-template <bool BF16, bool GELU>
-__device__ __forceinline__ uint32_t finish2(unsigned long long y) {
-  const float2 v = f2_split(GELU ? gelu2(y) : y);
-  if constexpr (BF16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
-    return *reinterpret_cast<const uint32_t*>(&h);
+// N pairs of outputs (with GELU) rounded to 16 bits, packed (the low half first).
+template <bool BF16, bool GELU, int N>
+__device__ __forceinline__ void finish2(unsigned long long (&y)[N], uint32_t (&w)[N]) {
+  if constexpr (GELU) gelu2(y);
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    const float2 v = f2_split(y[q]);
+    if constexpr (BF16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+      w[q] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      w[q] = pack_half2(v.x, v.y);
+    }
   }
-  return pack_half2(v.x, v.y);
 }
 
 template <bool BF16>
@@ -107,7 +136,8 @@ __device__ __forceinline__ float bias_f32(const uint16_t* b) {
 // (acc * a_scale) * w_scale + bias of two outputs, the same in both kernels (bit for bit)
 __device__ __forceinline__ unsigned long long dequant2(int acc0, int acc1, unsigned long long sa,
                                                        unsigned long long sw, unsigned long long bias) {
-  return f2_fma(f2_mul(f2(__int2float_rn(acc0), __int2float_rn(acc1)), sa), sw, bias);
+  const float2 a = f2_split(sa), w = f2_split(sw), b = f2_split(bias);
+  return f2(fmaf(__int2float_rn(acc0) * a.x, w.x, b.x), fmaf(__int2float_rn(acc1) * a.y, w.y, b.y));
 }
 
 // 32 lanes x 32 columns of TMEM, the load only; tmem_wait32 makes the registers valid.
@@ -133,38 +163,65 @@ __device__ __forceinline__ void tmem_wait32(int (&r)[32]) {
                : "memory");
 }
 
+// 16 lanes x 32 columns of TMEM in the 16x256b shape, the load only (tmem_wait16 makes the registers
+// valid): thread t gets rows t / 4 (r[4j], r[4j+1]) and t / 4 + 8 (r[4j+2], r[4j+3]) of columns
+// 8 j + 2 (t % 4) and the next, j = 0 .. 3.
+__device__ __forceinline__ void tmem_issue16(uint32_t taddr, int (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait16(int (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15])
+               :
+               : "memory");
+}
+
+// Four 8 x 8 matrices of 16-bit elements to shared memory: matrix i from w[i] of every thread (row t / 4,
+// elements 2 (t % 4) and the next), its row r at the address that lane 8 i + r gives.
+__device__ __forceinline__ void stmatrix4(uint32_t addr, const uint32_t (&w)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]),
+               "r"(w[2]), "r"(w[3])
+               : "memory");
+}
+
 // ====================================================================== many rows: SM pairs
 
-template <int BN>
+// COLS: columns per epilogue warp.
+template <int BN, int COLS>
 struct I8PairCfg {
   static constexpr int BM = 128;         // accumulator rows per CTA (256 per pair)
   static constexpr int B_ROWS = BN / 2;  // W rows held by each CTA
   static constexpr int A_BYTES = BM * kBK;
   static constexpr int B_BYTES = B_ROWS * kBK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int PARTS = BN / 64;  // epilogue warps per TMEM lane quadrant, 64 columns each
-  static constexpr int EPI_WARPS = 4 * PARTS;
+  static constexpr int EPI_WARPS = 4 * BN / COLS;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int STAGING_BYTES = EPI_WARPS * 4096;  // per epilogue warp: 32 rows x 128 B
-  static constexpr int COLS_BYTES = EPI_WARPS * 512;      // per epilogue warp: 64 scales, 64 biases
+  static constexpr int STAGING_BYTES = EPI_WARPS * 4096;   // per epilogue warp: two chunks of 16 rows x 64 columns
+  static constexpr int COLS_BYTES = EPI_WARPS * 8 * COLS;  // per epilogue warp: COLS scales and biases
   static constexpr int AUX_BYTES = 512 /*barriers*/ + COLS_BYTES;
-  static constexpr int RING_BYTES = 227 * 1024 - 1024 - STAGING_BYTES - AUX_BYTES;
-  static constexpr int STAGES = RING_BYTES / STAGE_BYTES;
+  static constexpr int STAGES = (227 * 1024 - 1024 - STAGING_BYTES - AUX_BYTES) / STAGE_BYTES;
   static constexpr int NACC = 2;
   static constexpr int TMEM_COLS = 512;
   static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + STAGING_BYTES + AUX_BYTES;
-  static_assert(BN % 64 == 0 && BN <= 256 && NACC * BN <= TMEM_COLS, "pair tile");
-  static_assert(STAGES >= 3 && SMEM <= 227 * 1024, "shared memory");
+  static_assert(BN % COLS == 0 && COLS % 64 == 0 && BN <= 256 && NACC * BN <= TMEM_COLS, "pair tile");
+  static_assert(STAGES >= 4 && SMEM <= 227 * 1024, "shared memory");
   static_assert((2 * STAGES + 2 * NACC) * 8 + 8 <= 512, "barriers");
 };
 
 // TMA_C: C is written with TMA stores (16-byte aligned rows); otherwise row by row from the
 // staging buffer with 2-byte stores, which any N and alignment allows.
-template <int BN, bool BF16, bool GELU, bool TMA_C>
-__global__ void __launch_bounds__(I8PairCfg<BN>::THREADS, 1)
+template <int BN, int COLS, bool BF16, bool GELU, bool TMA_C>
+__global__ void __launch_bounds__(I8PairCfg<BN, COLS>::THREADS, 1)
     linear_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                           const __grid_constant__ CUtensorMap tmC, const I8Params p) {
-  using Cfg = I8PairCfg<BN>;
+  using Cfg = I8PairCfg<BN, COLS>;
   constexpr int STAGES = Cfg::STAGES;
   constexpr int NACC = Cfg::NACC;
 
@@ -217,8 +274,22 @@ __global__ void __launch_bounds__(I8PairCfg<BN>::THREADS, 1)
   cluster_sync_all();  // both CTAs' barriers initialised, TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  auto tile_m0 = [&](int t) { return (t / n_tiles) * (2 * Cfg::BM) + half * Cfg::BM; };
-  auto tile_n0 = [&](int t) { return (t % n_tiles) * BN; };
+  // Tiles t in n-fastest order: rows m * 256 + 128 * half, columns n * BN.
+  struct Tile {
+    int t, m, n;
+  };
+  const int m_step = tile_step / n_tiles, n_step = tile_step % n_tiles;
+  const Tile tile0{first_tile, first_tile / n_tiles, first_tile % n_tiles};
+  auto next = [&](const Tile& c) {
+    Tile d{c.t + tile_step, c.m + m_step, c.n + n_step};
+    if (d.n >= n_tiles) {
+      d.n -= n_tiles;
+      ++d.m;
+    }
+    return d;
+  };
+  auto tile_m0 = [&](const Tile& c) { return c.m * (2 * Cfg::BM) + half * Cfg::BM; };
+  auto tile_n0 = [&](const Tile& c) { return c.n * BN; };
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
@@ -226,7 +297,7 @@ __global__ void __launch_bounds__(I8PairCfg<BN>::THREADS, 1)
       const uint32_t full0 = mapa_shared(smem_u32(full_bar), 0);
       int stage = 0;
       uint32_t phase = 0;
-      for (int tile = first_tile; tile < num_tiles && !*abort_flag; tile += tile_step) {
+      for (Tile tile = tile0; tile.t < num_tiles && !*abort_flag; tile = next(tile)) {
         const int m0 = tile_m0(tile);
         const int nb = tile_n0(tile) + half * Cfg::B_ROWS;
         for (int kb = 0; kb < k_blocks; ++kb) {
@@ -246,8 +317,6 @@ __global__ void __launch_bounds__(I8PairCfg<BN>::THREADS, 1)
     // ------------------------------------------------------------ MMA issuer (even CTA)
     if (leader && lane == 0) {
       constexpr uint32_t idesc = idesc_i8(2 * Cfg::BM, BN);
-      const uint32_t empty_peer = mapa_shared(smem_u32(empty_bar), 1);
-      const uint32_t accf_peer = mapa_shared(smem_u32(accf_bar), 1);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -269,16 +338,14 @@ __global__ void __launch_bounds__(I8PairCfg<BN>::THREADS, 1)
           for (int k = 0; k < kBK / kMmaK; ++k)
             tc_mma_i8_pair(d_tmem, sw128_kmajor_desc(a_addr + k * kMmaK), sw128_kmajor_desc(b_addr + k * kMmaK), idesc,
                            (kb | k) != 0 ? 1u : 0u);
-          tc_commit_pair(smem_u32(&empty_bar[stage]));
-          tc_commit_pair(empty_peer + stage * 8);
+          tc_commit_both(&empty_bar[stage]);  // the slot is free in both CTAs once these MMAs have read it
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
         if (!ok) break;
-        tc_commit_pair(smem_u32(&accf_bar[acc]));
-        tc_commit_pair(accf_peer + acc * 8);
+        tc_commit_both(&accf_bar[acc]);
         if (++acc == NACC) {
           acc = 0;
           acc_phase ^= 1;
@@ -288,91 +355,132 @@ __global__ void __launch_bounds__(I8PairCfg<BN>::THREADS, 1)
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int quad = warp & 3;         // TMEM lane quadrant this warp may access
-    const int part = (warp - 2) >> 2;  // which 64 columns of the tile
+    const int part = (warp - 2) >> 2;  // which COLS columns of the tile
     const int we = warp - 2;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
-    uint8_t* buf = s_stage + we * 4096;  // 32 rows x 64 columns, 16-byte piece c of row r at piece c ^ (r & 7)
-    float* s_sw = s_cols + we * 128;     // this warp's 64 channel scales, then 64 biases
-    float* s_b = s_sw + 64;
+    // Two chunks of 16 rows x 64 columns (row half 0 and 1), 16-byte piece c of row r at piece c ^ (r & 7).
+    uint8_t* buf = s_stage + we * 4096;
+    float* s_sw = s_cols + we * 2 * COLS;  // this warp's channel scales, then biases
+    float* s_b = s_sw + COLS;
     const uint32_t acce0 = mapa_shared(smem_u32(acce_bar), 0);
-    // The scales and biases of a tile are fetched while the previous tile is worked on (lane l:
-    // row l, columns l and 32 + l).
-    float sa_next = 0.f, sw_next[2] = {0.f, 0.f}, b_next[2] = {0.f, 0.f};
-    auto fetch = [&](int t) {
-      const int row = tile_m0(t) + quad * 32 + lane;
-      sa_next = row < p.M ? __ldg(p.a_scale + row) : 0.f;
+    const int row_t = lane >> 2, col_t = 2 * (lane & 3);  // this thread's place in an 8 x 8 block
+    // this lane's row and piece parity of the four blocks that one stmatrix4 writes: rows 0-7, 8-15 of a
+    // 16-byte piece, then of the next
+    const int row_m = (lane & 7) + (lane & 8), piece_m = lane >> 4;
+    // The scales and biases of a tile are fetched while the previous tile is worked on: the rows row_t + 8 i,
+    // and columns lane + 32 i for the warp's table.
+    float sa_next[4], sw_next[COLS / 32], b_next[COLS / 32];
+    auto fetch = [&](const Tile& t) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = tile_n0(t) + part * 64 + 32 * h + lane;
-        sw_next[h] = c < p.N ? __ldg(p.w_scale + c) : 0.f;
-        b_next[h] = p.bias && c < p.N ? bias_f32<BF16>(p.bias + c) : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        const int row = tile_m0(t) + quad * 32 + row_t + 8 * i;
+        sa_next[i] = row < p.M ? __ldg(p.a_scale + row) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < COLS / 32; ++i) {
+        const int c = tile_n0(t) + part * COLS + 32 * i + lane;
+        sw_next[i] = c < p.N ? __ldg(p.w_scale + c) : 0.f;
+        b_next[i] = p.bias && c < p.N ? bias_f32<BF16>(p.bias + c) : 0.f;
       }
     };
-    if (first_tile < num_tiles) fetch(first_tile);
+    if (first_tile < num_tiles) fetch(tile0);
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
+    Tile ahead = tile0;
+    for (Tile tile = tile0; tile.t < num_tiles; tile = ahead) {
       const int row0 = tile_m0(tile) + quad * 32;
-      const int c0 = tile_n0(tile) + part * 64;
-      if (TMA_C && lane == 0) bulk_wait_read<0>();  // the previous tile's store has read the buffer
-      __syncwarp();  // and its scales and biases have been read by every lane
-      const unsigned long long sa = f2(sa_next, sa_next);
+      const int c0 = tile_n0(tile) + part * COLS;
+      __syncwarp();  // every lane has read the previous tile's scales and biases
+      float sa[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s_sw[32 * h + lane] = sw_next[h];
-        s_b[32 * h + lane] = b_next[h];
+      for (int i = 0; i < 4; ++i) sa[i] = sa_next[i];
+#pragma unroll
+      for (int i = 0; i < COLS / 32; ++i) {
+        s_sw[32 * i + lane] = sw_next[i];
+        s_b[32 * i + lane] = b_next[i];
       }
       __syncwarp();
-      if (tile + tile_step < num_tiles) fetch(tile + tile_step);
+      ahead = next(tile);
+      if (ahead.t < num_tiles) fetch(ahead);
       if (!mbar_wait(&accf_bar[acc], acc_phase, abort_flag, &g_i8_err)) break;
       tc_fence_after();
-      const uint32_t tacc = tmem_base + lane_off + acc * BN + part * 64;
-      int v[2][32];
-      tmem_issue32(tacc, v[0]);
-      tmem_wait32(v[0]);
-      tmem_issue32(tacc + 32, v[1]);  // arrives while the first half is worked on
-      uint8_t* rowp = buf + lane * 128;
+      const uint32_t tacc = tmem_base + lane_off + acc * BN + part * COLS;
+      // steps of 16 rows x 32 columns (row half h of 32 columns, then the other half), the next one's
+      // TMEM load under way during each
+      constexpr int STEPS = COLS / 16;
+      int v[2][16];
+      tmem_issue16(tacc, v[0]);
+      unsigned long long sw[4], b[4];  // of this thread's 8 of the 32 columns
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (h == 1) {
-          tmem_wait32(v[1]);
+      for (int step = 0; step < STEPS; ++step) {
+        const int h = step & 1, cs = step >> 1;
+        tmem_wait16(v[step & 1]);
+        if (step < STEPS - 1) {
+          tmem_issue16(tacc + (static_cast<uint32_t>(16 * ((step + 1) & 1)) << 16) + 32 * ((step + 1) >> 1),
+                       v[(step + 1) & 1]);
+        } else {
           // accumulator read: release it to the even CTA's MMA thread
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(acce0 + acc * 8);
         }
+        if (h == 0) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+          for (int j = 0; j < 4; ++j) {
+            sw[j] = *reinterpret_cast<const unsigned long long*>(s_sw + 32 * cs + 8 * j + col_t);
+            b[j] = *reinterpret_cast<const unsigned long long*>(s_b + 32 * cs + 8 * j + col_t);
+          }
+        }
+        if (TMA_C && cs % 2 == 0) {
+          // the last store of this half's chunk has read it (half 1's was issued last)
+          if (lane == 0) {
+            if (h == 0) bulk_wait_read<1>();
+            else bulk_wait_read<0>();
+          }
+          __syncwarp();
+        }
+        const int(&x)[16] = v[step & 1];
+        const unsigned long long sa0 = f2(sa[2 * h], sa[2 * h]), sa1 = f2(sa[2 * h + 1], sa[2 * h + 1]);
+        const uint32_t dst = smem_u32(buf + h * 2048 + row_m * 128);
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          unsigned long long y[4];
           uint32_t w[4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int k = 8 * c + 4 * j;
-            const ulonglong2 sw = *reinterpret_cast<const ulonglong2*>(s_sw + 32 * h + k);
-            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + 32 * h + k);
-            w[2 * j] = finish2<BF16, GELU>(dequant2(v[h][k], v[h][k + 1], sa, sw.x, b.x));
-            w[2 * j + 1] = finish2<BF16, GELU>(dequant2(v[h][k + 2], v[h][k + 3], sa, sw.y, b.y));
+          for (int k = 0; k < 2; ++k) {
+            const int* a = &x[4 * (j + k)];
+            y[2 * k] = dequant2(a[0], a[1], sa0, sw[j + k], b[j + k]);
+            y[2 * k + 1] = dequant2(a[2], a[3], sa1, sw[j + k], b[j + k]);
           }
-          *reinterpret_cast<uint4*>(rowp + (((4 * h + c) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          finish2<BF16, GELU>(y, w);
+          stmatrix4(dst + (((4 * (cs & 1) + j + piece_m) ^ (lane & 7)) << 4), w);
         }
-      }
-      if constexpr (TMA_C) {
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0 && c0 < p.N && row0 < p.M) {
-          tma_store_2d(&tmC, buf, c0, row0);
-          bulk_commit();
-        }
-      } else {
-        // row by row: 32 neighbouring 2-byte stores at a time
-        __syncwarp();
-        const int rows = min(32, p.M - row0);
-        for (int r = 0; r < rows; ++r) {
+        if (cs % 2 == 1) {
+          // 16 rows x 64 columns are in place
+          const int col = c0 + 32 * (cs - 1), row = row0 + 16 * h;
+          if constexpr (TMA_C) {
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+              if (col < p.N && row < p.M) tma_store_2d(&tmC, buf + h * 2048, col, row);
+              bulk_commit();  // one group per chunk, empty ones too: bulk_wait_read counts them
+            }
+          } else {
+            // row by row: 32 neighbouring 2-byte stores at a time
+            __syncwarp();
+            const int rows = min(16, p.M - row);
+            for (int r = 0; r < rows; ++r) {
+              const uint8_t* line = buf + h * 2048 + r * 128;
+              uint16_t* c = p.C + static_cast<int64_t>(row + r) * p.ldc + col;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int col = 32 * h + lane;
-            const uint16_t o =
-                *reinterpret_cast<const uint16_t*>(buf + r * 128 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2);
-            if (c0 + col < p.N) p.C[static_cast<int64_t>(row0 + r) * p.ldc + c0 + col] = o;
+              for (int i = 0; i < 2; ++i) {
+                const int e = 32 * i + lane;
+                const uint16_t o =
+                    *reinterpret_cast<const uint16_t*>(line + (((e >> 3) ^ (r & 7)) << 4) + (e & 7) * 2);
+                if (col + e < p.N) c[e] = o;
+              }
+            }
+            __syncwarp();
           }
         }
       }
@@ -531,14 +639,15 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
   unsigned long long sw = 0, bias = 0;
   auto put4 = [&](int t, int4 a) {
     const ulonglong2 sa = *reinterpret_cast<const ulonglong2*>(s_sa + t);
-    const uint32_t w0 = finish2<BF16, GELU>(dequant2(a.x, a.y, sa.x, sw, bias));
-    const uint32_t w1 = finish2<BF16, GELU>(dequant2(a.z, a.w, sa.y, sw, bias));
+    unsigned long long y[2] = {dequant2(a.x, a.y, sa.x, sw, bias), dequant2(a.z, a.w, sa.y, sw, bias)};
+    uint32_t w[2];
+    finish2<BF16, GELU>(y, w);
     if (n < p.N) {
       uint16_t* c = p.C + static_cast<int64_t>(m0 + t) * p.ldc + n;
-      c[0] = static_cast<uint16_t>(w0);
-      if (t + 1 < tokens) c[p.ldc] = static_cast<uint16_t>(w0 >> 16);
-      if (t + 2 < tokens) c[2 * p.ldc] = static_cast<uint16_t>(w1);
-      if (t + 3 < tokens) c[3 * p.ldc] = static_cast<uint16_t>(w1 >> 16);
+      c[0] = static_cast<uint16_t>(w[0]);
+      if (t + 1 < tokens) c[p.ldc] = static_cast<uint16_t>(w[0] >> 16);
+      if (t + 2 < tokens) c[2 * p.ldc] = static_cast<uint16_t>(w[1]);
+      if (t + 3 < tokens) c[3 * p.ldc] = static_cast<uint16_t>(w[1] >> 16);
     }
   };
   // partial sums: int4 g (tokens 4 g ..) of channel ch from rank src at [src][ch][g], the 16-byte pieces of
@@ -667,9 +776,10 @@ struct I8Maps {
 
 template <int BN, bool BF16, bool GELU, bool TMA_C>
 cudaError_t launch_pair_i8(const I8Maps& m, const I8Params& p, int dev, int sms, cudaStream_t s) {
-  using Cfg = I8PairCfg<BN>;
+  constexpr int COLS = BN == 256 && !GELU ? 128 : 64;
+  using Cfg = I8PairCfg<BN, COLS>;
   static bool done[64] = {};
-  auto kern = linear_i8_pair_kernel<BN, BF16, GELU, TMA_C>;
+  auto kern = linear_i8_pair_kernel<BN, COLS, BF16, GELU, TMA_C>;
   const cudaError_t e = opt_in(kern, Cfg::SMEM, done, dev);
   if (e != cudaSuccess) return e;
   static int pairs_of[64] = {};
@@ -772,7 +882,7 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
     rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, bn / 2, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc)
-      rc = tma_c ? encode_2d_bytes(&maps.C, C, M, N, ldc, 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B)
+      rc = tma_c ? encode_2d_bytes(&maps.C, C, M, N, ldc, 2, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B)
                  : (maps.C = maps.A, BBH_OK);
     if (rc) return internal_fail(rc, "bbh_linear_i8: tensor map encoding failed");
     e = bn == 192 ? launch_pair_bn<192>(maps, p, bf16, g, tma_c, dev, sms, s)
