@@ -79,17 +79,16 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// erf-GELU, x Phi(x) = max(x, 0) - |x| Phi(-|x|), of N pairs of fp32 values (packed f32x2 fmas; the
-// pairs go through the polynomial side by side, which hides the fmas' latency and loads each
-// coefficient once). log2 Phi(-a) is close to a parabola and is evaluated as a polynomial of degree 10
-// in a (this project's own least-squares fit on [0, 5.75], reweighted to equal ripple; relative
-// error of Phi at most 2.2e-6, 3.3e-7 rms); beyond 5.75 the polynomial keeps falling, and Phi with it,
-// so no clamp is needed. |error| < 1e-6 max(|x|, 1) with ex2.approx's 2^-22.
+// erf-GELU, x Phi(x) = max(x, 0) - |x| Phi(-|x|), of N pairs of fp32 values side by side (which hides
+// the fmas' latency). log2 Phi(-a) is close to a parabola and is evaluated as a polynomial of degree 7
+// in a (this project's own least-squares fit on [0, 5.75], weighted by what an error means to the
+// output and reweighted to equal ripple): Phi(-a) is within 5.8e-6 of itself there (2.2e-6 rms);
+// beyond, the polynomial keeps falling, and Phi with it, so no clamp is needed. The output is within
+// 1e-6 max(|x|, 1), far inside its 16-bit rounding.
 template <int N>
 __device__ __forceinline__ void gelu2(unsigned long long (&x)[N]) {
-  constexpr float kPhi[11] = {-0.99999976158f,    -1.1511156559f,     -0.4591409266f,    -0.0526544638f,
-                              0.00723045366f,     -0.00021254165f,    -0.000184435105f,  5.04806158e-05f,
-                              -6.74621288e-06f,   4.83748636e-07f,    -1.48185313e-08f};
+  constexpr float kPhi[8] = {-0.999995351f,  -1.15125f,        -0.458468229f,   -0.0539548211f,
+                             0.00850458629f, -0.000929484435f, 6.14394376e-05f, -1.82546e-06f};
   float a[2 * N], p[2 * N];
 #pragma unroll
   for (int q = 0; q < N; ++q) {
@@ -99,9 +98,9 @@ __device__ __forceinline__ void gelu2(unsigned long long (&x)[N]) {
     x[q] = f2(fmaxf(r.x, 0.f), fmaxf(r.y, 0.f));
   }
 #pragma unroll
-  for (int q = 0; q < 2 * N; ++q) p[q] = fmaf(kPhi[10], a[q], kPhi[9]);
+  for (int q = 0; q < 2 * N; ++q) p[q] = fmaf(kPhi[7], a[q], kPhi[6]);
 #pragma unroll
-  for (int i = 8; i >= 0; --i)
+  for (int i = 5; i >= 0; --i)
 #pragma unroll
     for (int q = 0; q < 2 * N; ++q) p[q] = fmaf(p[q], a[q], kPhi[i]);
 #pragma unroll
@@ -136,8 +135,7 @@ __device__ __forceinline__ float bias_f32(const uint16_t* b) {
 // (acc * a_scale) * w_scale + bias of two outputs, the same in both kernels (bit for bit)
 __device__ __forceinline__ unsigned long long dequant2(int acc0, int acc1, unsigned long long sa,
                                                        unsigned long long sw, unsigned long long bias) {
-  const float2 a = f2_split(sa), w = f2_split(sw), b = f2_split(bias);
-  return f2(fmaf(__int2float_rn(acc0) * a.x, w.x, b.x), fmaf(__int2float_rn(acc1) * a.y, w.y, b.y));
+  return f2_fma(f2_mul(f2(__int2float_rn(acc0), __int2float_rn(acc1)), sa), sw, bias);
 }
 
 // 32 lanes x 32 columns of TMEM, the load only; tmem_wait32 makes the registers valid.
@@ -518,7 +516,7 @@ struct I8SmallCfg {
   static constexpr int B_BYTES = BN * kBK;   // BN tokens
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   // partial sums of the tokens that a CTA finishes, from every CTA of the cluster: int32
-  // [splits][128 channels][tokens], at least 4 tokens a CTA, at most 8 CTAs
+  // [splits][tokens / 4][128 channels][4], at least 4 tokens a CTA, at most 8 CTAs
   static constexpr int RED_BYTES = (BN < 32 ? 32 : BN) * 512;
   static constexpr int STAGES = (204 * 1024 - RED_BYTES) / STAGE_BYTES > 8 ? 8 : (204 * 1024 - RED_BYTES) / STAGE_BYTES;
   static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
@@ -637,24 +635,31 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
   const int ch = quad * 32 + lane;
   const int n = n0 + ch;
   unsigned long long sw = 0, bias = 0;
-  auto put4 = [&](int t, int4 a) {
-    const ulonglong2 sa = *reinterpret_cast<const ulonglong2*>(s_sa + t);
-    unsigned long long y[2] = {dequant2(a.x, a.y, sa.x, sw, bias), dequant2(a.z, a.w, sa.y, sw, bias)};
-    uint32_t w[2];
+  // G groups of four tokens from t on of this thread's channel: 2-byte stores, 32 neighbouring channels a
+  // warp (four channels a store, after a transposition between lanes, took longer). G groups side by
+  // side: the epilogue's time is the latency of its chain of steps.
+  auto put = [&](int t, const auto& a) {
+    constexpr int G = sizeof(a) / sizeof(int4);
+    unsigned long long y[2 * G];
+    uint32_t w[2 * G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const ulonglong2 sa = *reinterpret_cast<const ulonglong2*>(s_sa + t + 4 * g);
+      y[2 * g] = dequant2(a[g].x, a[g].y, sa.x, sw, bias);
+      y[2 * g + 1] = dequant2(a[g].z, a[g].w, sa.y, sw, bias);
+    }
     finish2<BF16, GELU>(y, w);
-    if (n < p.N) {
-      uint16_t* c = p.C + static_cast<int64_t>(m0 + t) * p.ldc + n;
-      c[0] = static_cast<uint16_t>(w[0]);
-      if (t + 1 < tokens) c[p.ldc] = static_cast<uint16_t>(w[0] >> 16);
-      if (t + 2 < tokens) c[2 * p.ldc] = static_cast<uint16_t>(w[1]);
-      if (t + 3 < tokens) c[3 * p.ldc] = static_cast<uint16_t>(w[1] >> 16);
+    uint16_t* c = p.C + static_cast<int64_t>(m0 + t) * p.ldc + n;
+    const int rows = n < p.N ? tokens - t : 0;
+#pragma unroll
+    for (int i = 0; i < 4 * G; ++i) {
+      if (i < rows) *c = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+      c += p.ldc;
     }
   };
-  // partial sums: int4 g (tokens 4 g ..) of channel ch from rank src at [src][ch][g], the 16-byte pieces of
-  // a channel permuted so that eight neighbouring channels' accesses fall into different banks
+  // partial sums: int4 g (tokens 4 g ..) of channel ch from rank src at [src][g][ch]
   const int log_per = max(2, (31 - __clz(BN)) - log_splits);  // tokens a CTA finishes: 2^log_per
   const int pieces = 1 << (log_per - 2);
-  const int swz = pieces >= 8 ? (ch & 7) : ((ch * pieces) >> 3) & (pieces - 1);
   bool ok = true;
   if (epi) {
     const int e = threadIdx.x - 64;
@@ -679,18 +684,25 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
       int v[32];
       tmem_issue32(tacc + c, v);
       tmem_wait32(v);
+      int4 a[8];
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        const int t = c + 4 * g;
-        const int4 a = make_int4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-        if (t < tokens) {
-          if (log_splits == 0) {
-            put4(t, a);
-          } else {
+      for (int g = 0; g < 8; ++g) a[g] = make_int4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+      if (log_splits == 0) {
+        if constexpr (BN >= 32) {
+          put(c, a);
+        } else {
+          const int4 low[4] = {a[0], a[1], a[2], a[3]};
+          put(c, low);
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const int t = c + 4 * g;
+          if (t < tokens) {
             const int piece = (t & ((1 << log_per) - 1)) >> 2;
-            const uint32_t at = smem_u32(red) + (((rank * 128 + ch) << log_per) << 2) + ((piece ^ swz) << 4);
+            const uint32_t at = smem_u32(red) + ((rank * pieces + piece) * 128 + ch) * 16;
             asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_shared(at, t >> log_per)),
-                         "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w)
+                         "r"(a[g].x), "r"(a[g].y), "r"(a[g].z), "r"(a[g].w)
                          : "memory");
           }
         }
@@ -702,21 +714,36 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
     cluster_arrive();
     cluster_wait();  // all partial sums are in place
     if (epi) {
-      for (int g = part; g < pieces; g += Cfg::PARTS) {
-        const int t = (rank << log_per) + 4 * g;
-        if (t >= tokens) break;
-        int4 a = make_int4(0, 0, 0, 0);
-#pragma unroll 1
-        for (int src = 0; src < splits; src += 2) {
-          const uint8_t* at = red + (((src * 128 + ch) << log_per) << 2) + ((g ^ swz) << 4);
-          const int4 x = *reinterpret_cast<const int4*>(at);
-          const int4 y = *reinterpret_cast<const int4*>(at + ((128 << log_per) << 2));
-          a.x += x.x + y.x;
-          a.y += x.y + y.y;
-          a.z += x.z + y.z;
-          a.w += x.w + y.w;
+      auto sum = [&](int g, auto& a) {
+        constexpr int G = sizeof(a) / sizeof(int4);
+#pragma unroll
+        for (int i = 0; i < G; ++i) a[i] = make_int4(0, 0, 0, 0);
+        for (int src = 0; src < splits; ++src) {
+          const int4* x = reinterpret_cast<const int4*>(red) + (src * pieces + g) * 128 + ch;
+#pragma unroll
+          for (int i = 0; i < G; ++i) {
+            const int4 u = x[i * 128];
+            a[i] = make_int4(a[i].x + u.x, a[i].y + u.y, a[i].z + u.z, a[i].w + u.w);
+          }
         }
-        put4(t, a);
+      };
+      const int mine = max(pieces / Cfg::PARTS, 1);  // this warp's pieces, from `first` on
+      const int first = part * mine;
+      const int t0 = rank << log_per;
+      if (first < pieces) {
+        if (mine >= 4) {
+          for (int g = first; g < first + mine && t0 + 4 * g < tokens; g += 4) {
+            int4 a[4];
+            sum(g, a);
+            put(t0 + 4 * g, a);
+          }
+        } else {
+          for (int g = first; g < first + mine && t0 + 4 * g < tokens; ++g) {
+            int4 a[1];
+            sum(g, a);
+            put(t0 + 4 * g, a);
+          }
+        }
       }
     }
   }
@@ -774,9 +801,8 @@ struct I8Maps {
   CUtensorMap A, W, C;
 };
 
-template <int BN, bool BF16, bool GELU, bool TMA_C>
+template <int BN, int COLS, bool BF16, bool GELU, bool TMA_C>
 cudaError_t launch_pair_i8(const I8Maps& m, const I8Params& p, int dev, int sms, cudaStream_t s) {
-  constexpr int COLS = BN == 256 && !GELU ? 128 : 64;
   using Cfg = I8PairCfg<BN, COLS>;
   static bool done[64] = {};
   auto kern = linear_i8_pair_kernel<BN, COLS, BF16, GELU, TMA_C>;
@@ -789,19 +815,28 @@ cudaError_t launch_pair_i8(const I8Maps& m, const I8Params& p, int dev, int sms,
   return launch_ex(kern, dim3(2 * pairs), dim3(Cfg::THREADS), Cfg::SMEM, s, true, 2, m.A, m.W, m.C, p);
 }
 
-template <int BN>
-cudaError_t launch_pair_bn(const I8Maps& m, const I8Params& p, bool bf16, bool gelu, bool tma_c, int dev, int sms,
-                           cudaStream_t s) {
-  switch ((bf16 ? 4 : 0) + (gelu ? 2 : 0) + (tma_c ? 1 : 0)) {
-    case 0: return launch_pair_i8<BN, false, false, false>(m, p, dev, sms, s);
-    case 1: return launch_pair_i8<BN, false, false, true>(m, p, dev, sms, s);
-    case 2: return launch_pair_i8<BN, false, true, false>(m, p, dev, sms, s);
-    case 3: return launch_pair_i8<BN, false, true, true>(m, p, dev, sms, s);
-    case 4: return launch_pair_i8<BN, true, false, false>(m, p, dev, sms, s);
-    case 5: return launch_pair_i8<BN, true, false, true>(m, p, dev, sms, s);
-    case 6: return launch_pair_i8<BN, true, true, false>(m, p, dev, sms, s);
-    default: return launch_pair_i8<BN, true, true, true>(m, p, dev, sms, s);
-  }
+template <int BN, int COLS, bool GELU>
+cudaError_t launch_pair_cols(const I8Maps& m, const I8Params& p, bool bf16, bool tma_c, int dev, int sms,
+                             cudaStream_t s) {
+  if (bf16)
+    return tma_c ? launch_pair_i8<BN, COLS, true, GELU, true>(m, p, dev, sms, s)
+                 : launch_pair_i8<BN, COLS, true, GELU, false>(m, p, dev, sms, s);
+  return tma_c ? launch_pair_i8<BN, COLS, false, GELU, true>(m, p, dev, sms, s)
+               : launch_pair_i8<BN, COLS, false, GELU, false>(m, p, dev, sms, s);
+}
+
+// Epilogue warps of the 256-wide tile: eight of 128 columns leave room for a fifth stage; sixteen of 64
+// columns finish a tile sooner, which counts when the GELU takes longer than the tile's MMAs: 8192 x
+// 4096 with GELU, K = 384: 24.8 us with sixteen, 28.4 with eight; K = 768: 30.0 / 29.5; K = 4096: 94.1 /
+// 89.7. Without GELU eight are as fast at K = 384 (50.5 us for 68451 x 1536) and faster above.
+cudaError_t launch_pair_any(const I8Maps& m, const I8Params& p, int bn, bool bf16, bool gelu, bool tma_c, int dev,
+                            int sms, cudaStream_t s) {
+  if (bn == 192)
+    return gelu ? launch_pair_cols<192, 64, true>(m, p, bf16, tma_c, dev, sms, s)
+                : launch_pair_cols<192, 64, false>(m, p, bf16, tma_c, dev, sms, s);
+  if (!gelu) return launch_pair_cols<256, 128, false>(m, p, bf16, tma_c, dev, sms, s);
+  return p.K >= 768 ? launch_pair_cols<256, 128, true>(m, p, bf16, tma_c, dev, sms, s)
+                    : launch_pair_cols<256, 64, true>(m, p, bf16, tma_c, dev, sms, s);
 }
 
 template <int BN, bool BF16, bool GELU>
@@ -823,6 +858,40 @@ cudaError_t launch_small_bn(const I8Maps& m, const I8Params& p, bool bf16, bool 
                 : launch_small_i8<BN, true, false>(m, p, log_splits, dev, s);
   return gelu ? launch_small_i8<BN, false, true>(m, p, log_splits, dev, s)
               : launch_small_i8<BN, false, false>(m, p, log_splits, dev, s);
+}
+
+struct I8Plan {
+  bool pair;
+  int bn;          // column tile of the pair kernel, token tile of the other
+  int log_splits;  // K split over 2^log_splits CTAs
+};
+
+// The kernel and tile that take the least time by this model of a launch, in us, fitted to times of
+// back-to-back launches on a B200 (sizes from 16 to 2048 rows, 384 to 8192 columns, K to 8192; it is
+// within about 10 % of them and picks the fastest or one within 5 % of it):
+//   few rows: 1.65 + 0.0113 bn + 0.235 k-blocks per CTA, and 0.7 + 0.008 bn log2(splits) for a split K (the
+//     cluster's barriers and the exchange of partial sums), every CTA on an SM of its own;
+//   pairs: 3.9 + 0.28 k-blocks per round of tiles.
+// E.g. 64 x 4096 x 4096: bn 64 in 4 parts 6.1 us, bn 32 in 2 parts 6.8, bn 64 whole 9.9, pairs 12.7;
+// 1000 x 1000 x 1000: bn 64 whole 5.0 us, bn 128 in 2 parts 6.3, pairs 7.7.
+I8Plan choose_plan(int M, int N, int K, int sms) {
+  const int k_blocks = (K + kBK - 1) / kBK;
+  const int64_t ch_tiles = (N - 1) / 128 + 1;
+  const int bn2 = N % 256 && N % 192 == 0 ? 192 : 256;
+  const int64_t tiles2 = (int64_t(M) + 255) / 256 * ((N - 1) / bn2 + 1);
+  I8Plan best{true, bn2, 0};
+  double best_us = 3.9 + 0.28 * k_blocks * static_cast<double>((tiles2 - 1) / (sms / 2) + 1);
+  for (int bn = 16; bn <= 128; bn *= 2) {
+    const int64_t tiles = ch_tiles * ((int64_t(M) + bn - 1) / bn);
+    for (int ls = 0; ls <= 3 && (tiles << ls) <= sms && (1 << ls) <= k_blocks; ++ls) {
+      const double us = 1.65 + 0.0113 * bn + 0.235 * ((k_blocks + (1 << ls) - 1) >> ls) + (ls ? 0.7 + 0.008 * bn * ls : 0);
+      if (us < best_us) {
+        best_us = us;
+        best = {false, bn, ls};
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -861,32 +930,25 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   I8Maps maps;
   cudaError_t e;
-  const int ch_tiles = (N - 1) / 128 + 1;
-  const int64_t small128 = int64_t(ch_tiles) * ((M - 1) / 128 + 1);
-  if (small128 <= sms) {
-    // few rows
-    const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int k_blocks = (K + kBK - 1) / kBK;
-    const int tiles = ch_tiles * ((M - 1) / bn + 1);
-    int log_splits = 0;
-    while (log_splits < 3 && (tiles << (log_splits + 1)) <= sms && (2 << log_splits) <= k_blocks) ++log_splits;
+  const I8Plan plan = choose_plan(M, N, K, sms);
+  if (!plan.pair) {
     rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, bn, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, plan.bn, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return internal_fail(rc, "bbh_linear_i8: tensor map encoding failed");
-    e = bn == 16   ? launch_small_bn<16>(maps, p, bf16, g, log_splits, dev, s)
-        : bn == 32 ? launch_small_bn<32>(maps, p, bf16, g, log_splits, dev, s)
-        : bn == 64 ? launch_small_bn<64>(maps, p, bf16, g, log_splits, dev, s)
-                   : launch_small_bn<128>(maps, p, bf16, g, log_splits, dev, s);
+    switch (plan.bn) {
+      case 16: e = launch_small_bn<16>(maps, p, bf16, g, plan.log_splits, dev, s); break;
+      case 32: e = launch_small_bn<32>(maps, p, bf16, g, plan.log_splits, dev, s); break;
+      case 64: e = launch_small_bn<64>(maps, p, bf16, g, plan.log_splits, dev, s); break;
+      default: e = launch_small_bn<128>(maps, p, bf16, g, plan.log_splits, dev, s); break;
+    }
   } else {
-    const int bn = N % 256 && N % 192 == 0 ? 192 : 256;
     rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, bn / 2, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, plan.bn / 2, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc)
       rc = tma_c ? encode_2d_bytes(&maps.C, C, M, N, ldc, 2, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B)
                  : (maps.C = maps.A, BBH_OK);
     if (rc) return internal_fail(rc, "bbh_linear_i8: tensor map encoding failed");
-    e = bn == 192 ? launch_pair_bn<192>(maps, p, bf16, g, tma_c, dev, sms, s)
-                  : launch_pair_bn<256>(maps, p, bf16, g, tma_c, dev, sms, s);
+    e = launch_pair_any(maps, p, plan.bn, bf16, g, tma_c, dev, sms, s);
   }
   if (e != cudaSuccess) return internal_fail(BBH_ERR_CUDA, std::string("bbh_linear_i8: ") + cudaGetErrorString(e));
   return BBH_OK;

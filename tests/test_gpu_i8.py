@@ -290,8 +290,8 @@ def test_linear_i8(M, N, K, dtype):
 @pytest.mark.parametrize("M,N,K", [(3, 200, 96), (64, 384, 384), (300, 513, 384), (3000, 1536, 384), (2500, 1341, 64),
                                    (2600, 1152, 384)])
 def test_linear_i8_gelu(M, N, K, dtype):
-    """x Phi(x) = max(x, 0) - |x| Phi(-|x|): Phi(-|x|) is within 2.2e-6 of itself by its fit and 2^-21 by
-    ex2, in all 3e-6; the input's error (as without GELU) grows by the GELU's steepest slope, 1.13; two
+    """x Phi(x) = max(x, 0) - |x| Phi(-|x|): Phi(-|x|) is within 5.8e-6 of itself by its fit and 2^-21 by
+    ex2, in all 6.3e-6; the input's error (as without GELU) grows by the GELU's steepest slope, 1.13; two
     fp32 roundings follow, then the 16-bit one."""
     import bbh
 
@@ -300,7 +300,7 @@ def test_linear_i8_gelu(M, N, K, dtype):
     p, z = linear64(a, sa, w, sw, b)
     tail = 0.5 * torch.special.erfc(z.abs() / 2**0.5)
     want = z.clamp(min=0) - z.abs() * tail
-    tol = 1.13 * U * (2 * p.abs() + z.abs()) + 3e-6 * z.abs() * tail + (2 * U + HALF[dtype]) * want.abs() + TINY[dtype]
+    tol = 1.13 * U * (2 * p.abs() + z.abs()) + 6.3e-6 * z.abs() * tail + (2 * U + HALF[dtype]) * want.abs() + TINY[dtype]
     err = (c.double() - want).abs()
     assert bool((err <= tol * (1 + 1e-6)).all()), f"{(err / tol).max().item():.3f} of the tolerance"
 
@@ -321,7 +321,7 @@ def test_linear_i8_gelu_over_the_range():
         tail = 0.5 * torch.special.erfc(z.abs() / 2**0.5)
         want = z.clamp(min=0) - z.abs() * tail
         # beyond the fit's 5.75 Phi is only known to be small: |x| Phi(-|x|) < 2e-8 there
-        tol = 3e-6 * z.abs() * tail + (2 * U + HALF[dtype]) * want.abs() + TINY[torch.float16]
+        tol = 6.3e-6 * z.abs() * tail + (2 * U + HALF[dtype]) * want.abs() + TINY[torch.float16]
         assert bool(((c[:-1].double() - want).abs() <= tol).all())
         assert bool(torch.isnan(c[-1]))
 
