@@ -35,6 +35,7 @@ struct RowParams {
   int rows, D;
   int group;  // threads of a row: a power of two, 16 .. 512
   float eps;
+  float inv_D;  // 1 / D
 };
 
 constexpr int kRowBlock = 128;  // threads of a block when a row takes fewer
@@ -54,198 +55,311 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   return pack_half2(a, b);
 }
 
-// max that keeps a NaN of either side (fmaxf drops it)
+// max(m, |a|, |b|) that keeps a NaN of any of them (fmaxf drops it)
+__device__ __forceinline__ float max_abs_nan(float m, float a, float b) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-
-// A thread's 8 values of chunk j. VEC 8: eight consecutive elements, one 16-byte access
-// (rows 16-byte aligned, D a multiple of 8). VEC 1: elements a group's width apart, 2-byte
-// accesses, which any alignment and width allows.
-template <int VEC>
-__device__ __forceinline__ int elem(int j, int i, int t, int group) {
-  return VEC == 8 ? 8 * (j * group + t) + i : (8 * j + i) * group + t;
+// the same on a packed pair of 16-bit values
+template <bool BF16>
+__device__ __forceinline__ uint32_t max_abs_nan2(uint32_t m, uint32_t w) {
+  uint32_t a = w & 0x7fff7fffu, d;
+  if constexpr (BF16)
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(m), "r"(a));
+  else
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(m), "r"(a));
+  return d;
 }
 
-template <int VEC>
-__device__ __forceinline__ uint4 load8(const uint16_t* row, int j, int t, int group, int D) {
-  uint4 u = make_uint4(0, 0, 0, 0);
-  if constexpr (VEC == 8) {
-    const int e = elem<8>(j, 0, t, group);
-    if (e < D) u = *reinterpret_cast<const uint4*>(row + e);
+// How a row is cut into the 8-element chunks of its threads; chunk c = j * group + t is thread t's j-th.
+//  kAligned  chunk c is elements 8c .. 8c + 7, one 16-byte access: rows 16-byte aligned, D a multiple of 8.
+//  kShifted  the 16-bit tensors' rows start `sh` elements behind a 16-byte boundary, the same for all of
+//            them (contiguous tensors of any width are so): chunk c is elements 8c - sh .. 8c - sh + 7, which
+//            is one 16-byte access inside the row; the row's first and last chunk go element by element.
+//  kSingle   any strides and alignments: elements `group` apart, 2-byte accesses.
+enum Cut : int { kAligned, kShifted, kSingle };
+
+template <int CUT>
+__device__ __forceinline__ int elem(int j, int i, int t, int group, int sh) {
+  if (CUT == kSingle) return (8 * j + i) * group + t;
+  return 8 * (j * group + t) + i - (CUT == kShifted ? sh : 0);
+}
+
+// Elements e .. e + 7 one by one, zeros outside [0, D).
+__device__ __forceinline__ uint4 load_edge(const uint16_t* row, int e, int D) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (e + 8 > 0 && e < D) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e + i >= 0 && e + i < D) w[i >> 1] |= static_cast<uint32_t>(row[e + i]) << (16 * (i & 1));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int CUT>
+__device__ __forceinline__ uint4 load8(const uint16_t* row, int j, int t, int group, int sh, int D) {
+  const int e = elem<CUT>(j, 0, t, group, sh);
+  if constexpr (CUT == kAligned) {
+    return e < D ? *reinterpret_cast<const uint4*>(row + e) : make_uint4(0, 0, 0, 0);
+  } else if constexpr (CUT == kShifted) {
+    return e >= 0 && e + 8 <= D ? *reinterpret_cast<const uint4*>(row + e) : load_edge(row, e, D);
   } else {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int e = elem<1>(j, i, t, group);
-      if (e < D) w[i >> 1] |= static_cast<uint32_t>(row[e]) << (16 * (i & 1));
+      const int k = elem<kSingle>(j, i, t, group, 0);
+      if (k < D) w[i >> 1] |= static_cast<uint32_t>(row[k]) << (16 * (i & 1));
     }
-    u = make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  return u;
 }
 
-template <int VEC, bool BF16>
-__device__ __forceinline__ void store8(uint16_t* row, int j, int t, int group, int D, const float* f) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack16<BF16>(f[2 * i], f[2 * i + 1]);
-  if constexpr (VEC == 8) {
-    const int e = elem<8>(j, 0, t, group);
-    if (e < D) *reinterpret_cast<uint4*>(row + e) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
+template <int CUT>
+__device__ __forceinline__ void store8(uint16_t* row, int j, int t, int group, int sh, int D, uint4 u) {
+  const int e = elem<CUT>(j, 0, t, group, sh);
+  if (CUT == kAligned) {
+    if (e < D) *reinterpret_cast<uint4*>(row + e) = u;
+    return;
+  }
+  if (CUT == kShifted && e >= 0 && e + 8 <= D) {
+    *reinterpret_cast<uint4*>(row + e) = u;
+    return;
+  }
+  if (CUT == kSingle || (e + 8 > 0 && e < D)) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int e = elem<1>(j, i, t, group);
-      if (e < D) row[e] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+      const int k = elem<CUT>(j, i, t, group, sh);
+      if (k >= 0 && k < D) row[k] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
     }
   }
 }
 
-// rint(f * 127 / top) as the low byte of f * inv + 1.5 * 2^23 (rounded half to even there);
-// |f * inv| <= 127 (1 + 2^-23), which rounds to 127 at most. Elements of a 16-bit row meet exact
-// halves (top / 2 is 63.5 steps), which inv = 127 / top rounded to fp32 would push to either
-// side: TIES adds the rest of 127 / top, so that f * 127 / top is right to fp32 and a half
-// stays one (with 11-bit elements every other value is 2^-20 of itself or more away from a half).
-template <bool TIES>
-__device__ __forceinline__ uint32_t round_byte(float f, float inv, float inv_rest) {
-  if constexpr (TIES) return __float_as_uint(fmaf(f, inv, f * inv_rest) + 12582912.f);
-  return __float_as_uint(fmaf(f, inv, 12582912.f));
+// A chunk of the weight, whose start is 16-byte aligned where the rows' is not (kShifted): the eight
+// elements lie in two neighbouring 16-byte pieces, taken out of their eight words by `sh`.
+template <int CUT>
+__device__ __forceinline__ uint4 load_weight8(const uint16_t* weight, int j, int t, int group, int sh, int D) {
+  if (CUT != kShifted || sh == 0) return load8<CUT>(weight, j, t, group, sh, D);
+  const int c = j * group + t;  // elements 8c - sh ..: the end of piece c - 1, the start of piece c
+  if (c == 0 || 8 * c + 8 > D) return load_edge(weight, 8 * c - sh, D);
+  const uint4 lo = *reinterpret_cast<const uint4*>(weight + 8 * c - 8);
+  const uint4 hi = *reinterpret_cast<const uint4*>(weight + 8 * c);
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  const int words = (8 - sh) >> 1;  // 0 .. 3
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = words & 2 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = words & 1 ? w[i + 1] : w[i];
+  const uint32_t pick = sh & 1 ? 0x5432u : 0x3210u;
+  return make_uint4(__byte_perm(w[0], w[1], pick), __byte_perm(w[1], w[2], pick), __byte_perm(w[2], w[3], pick),
+                    __byte_perm(w[3], w[4], pick));
 }
 
-template <int VEC, bool TIES>
-__device__ __forceinline__ void store_q8(int8_t* row, int j, int t, int group, int D, const float* f, float inv,
-                                         float inv_rest) {
+template <bool BF16>
+__device__ __forceinline__ void unpack8(uint4 u, float* f) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = unpack16<BF16>(w[i]);
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 pack8(const float* f) {
+  return make_uint4(pack16<BF16>(f[0], f[1]), pack16<BF16>(f[2], f[3]), pack16<BF16>(f[4], f[5]),
+                    pack16<BF16>(f[6], f[7]));
+}
+
+// The low bytes of eight words.
+__device__ __forceinline__ uint2 low_bytes(const uint32_t* b) {
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+
+// rint(f * 127 / top) of eight values as bytes: the low byte of f * inv + 1.5 * 2^23, one fma that
+// rounds half to even. inv is 127 / top rounded up; f * inv <= 127 (1 + 2^-22), which rounds to 127.
+//
+// Elements of a 16-bit row (kRowQuant) meet exact halves, which a rounded inv would push to either
+// side. If 127 does not divide top's significand the only one is |f| = top / 2, 63.5 steps, and inv rounded
+// up takes it to 64, the even neighbour (other values are 2^-20 of themselves or more away from a
+// half). If 127 divides it (`ties`), f * inv + f * rest, with rest what inv lacks of 127 / top, is right
+// to fp32 and a half stays one.
+__device__ __forceinline__ uint2 quantize8(const float* f, float inv, float rest, bool ties) {
   uint32_t b[8];
+  if (ties) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) b[i] = inv > 0.f ? round_byte<TIES>(f[i], inv, inv_rest) : 0u;
-  if constexpr (VEC == 8) {
-    const int e = elem<8>(j, 0, t, group);
-    uint2 o;
-    o.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-    o.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-    if (e < D) *reinterpret_cast<uint2*>(row + e) = o;
+    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(fmaf(f[i], inv, f[i] * rest) + 12582912.f);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int e = elem<1>(j, i, t, group);
-      if (e < D) row[e] = static_cast<int8_t>(b[i]);
-    }
+    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(fmaf(f[i], inv, 12582912.f));
   }
+  return low_bytes(b);
 }
 
-// Sum of s and maximum of m over the `group` threads of a row (a power of two; groups of more
-// than a warp exchange through shared memory). Every thread of the block calls it.
+// Sum of s and maximum of m over the `group` threads of a row (a power of two from 16 on; groups of
+// more than a warp exchange through shared memory). Every thread of the block calls it.
 template <bool SUM, bool MAX>
 __device__ __forceinline__ void group_reduce(float& s, float& m, int group) {
   __shared__ float2 part[kRowMaxBlock / 32];
-  const int lane = threadIdx.x & 31;
-  const int width = group < 32 ? group : 32;
-  for (int o = width >> 1; o > 0; o >>= 1) {
+  auto step = [&](int o) {
     if (SUM) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (MAX) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  }
+  };
+  if (group > 16) step(16);
+  step(8);
+  step(4);
+  step(2);
+  step(1);
   if (group > 32) {
-    const int warps = group >> 5;
-    const int warp = threadIdx.x >> 5;
+    const int warps = group >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) part[warp] = make_float2(s, m);
     __syncthreads();
     const float2 p = part[(warp & ~(warps - 1)) + (lane & (warps - 1))];
     s = p.x;
     m = p.y;
-    for (int o = warps >> 1; o > 0; o >>= 1) {
-      if (SUM) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (MAX) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    }
+    if (warps > 8) step(8);
+    if (warps > 4) step(4);
+    if (warps > 2) step(2);
+    step(1);
   }
 }
 
-// V: 8-element chunks a thread holds (D <= 8 * V * group).
-template <int MODE, bool BF16, int V, int VEC>
-__global__ void __launch_bounds__(kRowMaxBlock) row_kernel(const RowParams p) {
+// V: 8-element chunks a thread holds. 64 registers up to four chunks (32 warps an SM: with 82, norm of
+// 8192 x 4096 took 27.1 us instead of 22.9).
+template <int MODE, bool BF16, int V, int CUT>
+__global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1) row_kernel(const RowParams p) {
   pdl_launch_dependents();
   const int group = p.group;
   const int t = threadIdx.x & (group - 1);
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
   const bool live = r < p.rows;
   const int D = live ? p.D : 0;  // a group behind the last row loads and stores nothing
+  const uint16_t* x = p.x + r * p.ldx;
+  const int sh = CUT == kShifted ? static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) >> 1 : 0;
   pdl_wait();
 
-  uint4 ux[V], ur[V], uw[V];
+  uint4 ux[V], ur[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) ux[j] = load8<VEC>(p.x + r * p.ldx, j, t, group, D);
+  for (int j = 0; j < V; ++j) ux[j] = load8<CUT>(x, j, t, group, sh, D);
   if (MODE != kRowQuant && p.residual) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) ur[j] = load8<VEC>(p.residual + r * p.ldr, j, t, group, D);
-  }
-  if (MODE != kRowQuant && p.weight) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) uw[j] = load8<VEC>(p.weight, j, t, group, D);
+    for (int j = 0; j < V; ++j) ur[j] = load8<CUT>(p.residual + r * p.ldr, j, t, group, sh, D);
   }
 
   float f[8 * V];
   float ss = 0.f, top = 0.f;
+  uint32_t top2 = 0;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float* v = f + 8 * j;
-    const uint32_t* a = reinterpret_cast<const uint32_t*>(&ux[j]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 u = unpack16<BF16>(a[i]);
-      v[2 * i] = u.x;
-      v[2 * i + 1] = u.y;
-    }
-    if constexpr (MODE != kRowQuant) {
+    unpack8<BF16>(ux[j], v);
+    if constexpr (MODE == kRowQuant) {
+      top2 = max_abs_nan2<BF16>(top2, ux[j].x);
+      top2 = max_abs_nan2<BF16>(top2, ux[j].y);
+      top2 = max_abs_nan2<BF16>(top2, ux[j].z);
+      top2 = max_abs_nan2<BF16>(top2, ux[j].w);
+    } else {
       if (p.residual) {
-        const uint32_t* b = reinterpret_cast<const uint32_t*>(&ur[j]);
+        float u[8];
+        unpack8<BF16>(ur[j], u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 u = unpack16<BF16>(b[i]);
-          v[2 * i] += u.x;
-          v[2 * i + 1] += u.y;
-        }
-        if (p.sum) store8<VEC, BF16>(p.sum + r * p.lds, j, t, group, D, v);
+        for (int i = 0; i < 8; ++i) v[i] += u[i];
+        if (p.sum) store8<CUT>(p.sum + r * p.lds, j, t, group, sh, D, pack8<BF16>(v));
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-      if (p.weight) {
-        const uint32_t* b = reinterpret_cast<const uint32_t*>(&uw[j]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 u = unpack16<BF16>(b[i]);
-          v[2 * i] *= u.x;
-          v[2 * i + 1] *= u.y;
-        }
-      }
     }
-    if constexpr (MODE != kRowNorm) {
+    if constexpr (MODE == kRowNormI8) {
+      if (p.weight) {
+        float u[8];
+        unpack8<BF16>(load_weight8<CUT>(p.weight, j, t, group, sh, D), u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
+        for (int i = 0; i < 8; ++i) v[i] *= u[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) top = max_abs_nan(top, v[i], v[i + 1]);
     }
   }
+  if constexpr (MODE == kRowQuant) {
+    const float2 m = unpack16<BF16>(top2);
+    top = max_nan(m.x, m.y);
+  }
   group_reduce<MODE != kRowQuant, MODE != kRowNorm>(ss, top, group);
-  const float rstd = MODE == kRowQuant ? 1.f : rsqrtf(ss / static_cast<float>(p.D) + p.eps);
+  const float rstd = MODE == kRowQuant ? 1.f : rsqrtf(ss * p.inv_D + p.eps);
 
   if constexpr (MODE == kRowNorm) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      float* v = f + 8 * j;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[8 * j + i] *= rstd;
-      store8<VEC, BF16>(p.y + r * p.ldy, j, t, group, D, f + 8 * j);
+      for (int i = 0; i < 8; ++i) v[i] *= rstd;
+      if (p.weight) {
+        float u[8];
+        unpack8<BF16>(load_weight8<CUT>(p.weight, j, t, group, sh, D), u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= u[i];
+      }
+      store8<CUT>(p.y + r * p.ldy, j, t, group, sh, D, pack8<BF16>(v));
     }
   } else {
     // A row whose largest magnitude is below 2^-120 (127 / top would near the end of fp32) is
     // stored as zeros with scale 0; one with a NaN or an infinity as zeros with scale NaN, so
     // that whatever is computed from it is NaN too.
     const bool finite = top <= FLT_MAX;
-    const float inv = finite && top >= 0x1p-120f ? 127.f / top : 0.f;
-    const float rest = inv > 0.f ? fmaf(-inv, top, 127.f) / top : 0.f;
-    if (live && t == 0)
-      p.scale[r] = finite ? (inv > 0.f ? top / 127.f : 0.f) * rstd : __int_as_float(0x7fc00000);
+    const bool zero = !finite || top < 0x1p-120f;
+    const float inv = __fdiv_ru(127.f, zero ? 1.f : top);
+    bool ties = false;
+    float rest = 0.f;
+    if constexpr (MODE == kRowQuant) {
+      ties = (((__float_as_uint(top) >> 13) & 0x3ffu) | 0x400u) % 127u == 0;
+      if (ties) rest = fmaf(-inv, top, 127.f) / top;
+    }
+    if (live && t == 0) p.scale[r] = finite ? (zero ? 0.f : top / 127.f) * rstd : __int_as_float(0x7fc00000);
+    int8_t* q = p.q + r * p.ldq;
+    if constexpr (CUT == kShifted) {
+      // The bytes of a chunk are not where an aligned store of q wants them: through shared memory. The
+      // rows of q are 8-byte aligned.
+      extern __shared__ uint2 s_q[];
+      uint2* row = s_q + (threadIdx.x / group) * (V * group + 1);
 #pragma unroll
-    for (int j = 0; j < V; ++j) store_q8<VEC, MODE == kRowQuant>(p.q + r * p.ldq, j, t, group, D, f + 8 * j, inv, rest);
+      for (int j = 0; j < V; ++j) row[j * group + t] = quantize8(f + 8 * j, inv, rest, ties);
+      if (t == 0) row[V * group] = make_uint2(0, 0);
+      __syncthreads();
+      for (int c = t; 8 * c < D; c += group) {  // elements 8c ..: bytes sh .. of chunk c, then of chunk c + 1
+        const uint2 a = row[c], b = row[c + 1];
+        const uint64_t lo = static_cast<uint64_t>(a.y) << 32 | a.x, hi = static_cast<uint64_t>(b.y) << 32 | b.x;
+        uint64_t o = sh ? lo >> (8 * sh) | hi << (64 - 8 * sh) : lo;
+        if (zero) o = 0;
+        if (8 * c + 8 <= D) {
+          *reinterpret_cast<uint64_t*>(q + 8 * c) = o;
+        } else {
+          for (int i = 0; 8 * c + i < D; ++i) q[8 * c + i] = static_cast<int8_t>(o >> (8 * i));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        uint2 o = quantize8(f + 8 * j, inv, rest, ties);
+        if (zero) o = make_uint2(0, 0);
+        const int e = elem<CUT>(j, 0, t, group, 0);
+        if constexpr (CUT == kAligned) {
+          if (e < D) *reinterpret_cast<uint2*>(q + e) = o;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int k = elem<kSingle>(j, i, t, group, 0);
+            if (k < D) q[k] = static_cast<int8_t>((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
+          }
+        }
+      }
+    }
   }
 }
 
@@ -258,7 +372,20 @@ struct DequantParams {
   int rows, D, group;
 };
 
-template <bool BF16, int VEC>
+// Eight bytes of q from element e on, where q + e is `sh` bytes before an 8-byte boundary.
+__device__ __forceinline__ uint2 load_q8(const int8_t* q, int e, int sh, int D) {
+  uint64_t o = 0;
+  if (e >= 0 && e + sh + 8 <= D) {
+    const uint64_t hi = *reinterpret_cast<const uint64_t*>(q + e + sh);
+    o = sh ? *reinterpret_cast<const uint64_t*>(q + e + sh - 8) >> (64 - 8 * sh) | hi << (8 * sh) : hi;
+  } else {
+    for (int i = 0; i < 8; ++i)
+      if (e + i >= 0 && e + i < D) o |= static_cast<uint64_t>(static_cast<uint8_t>(q[e + i])) << (8 * i);
+  }
+  return make_uint2(static_cast<uint32_t>(o), static_cast<uint32_t>(o >> 32));
+}
+
+template <bool BF16, int CUT>
 __global__ void __launch_bounds__(kRowMaxBlock) dequant_kernel(const DequantParams p) {
   pdl_launch_dependents();
   const int group = p.group;
@@ -268,21 +395,24 @@ __global__ void __launch_bounds__(kRowMaxBlock) dequant_kernel(const DequantPara
   if (r >= p.rows) return;
   const int8_t* q = p.q + r * p.ldq;
   uint16_t* y = p.y + r * p.ldy;
+  const int sh = CUT == kShifted ? static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) >> 1 : 0;
   const float s = p.scale[r];
-  for (int j0 = 0; elem<VEC>(j0, 0, t, group) < p.D; j0 += 4) {
+  for (int j0 = 0; elem<CUT>(j0, 0, t, group, sh) < p.D; j0 += 4) {
     uint2 u[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      const int e = elem<CUT>(j0 + k, 0, t, group, sh);
       u[k] = make_uint2(0, 0);
-      if constexpr (VEC == 8) {
-        const int e = elem<8>(j0 + k, 0, t, group);
+      if constexpr (CUT == kAligned) {
         if (e < p.D) u[k] = *reinterpret_cast<const uint2*>(q + e);
+      } else if constexpr (CUT == kShifted) {
+        if (e < p.D) u[k] = load_q8(q, e, sh, p.D);
       } else {
         uint32_t w[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int e = elem<1>(j0 + k, i, t, group);
-          if (e < p.D) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(q[e])) << (8 * (i & 3));
+          const int m = elem<kSingle>(j0 + k, i, t, group, 0);
+          if (m < p.D) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(q[m])) << (8 * (i & 3));
         }
         u[k] = make_uint2(w[0], w[1]);
       }
@@ -295,7 +425,7 @@ __global__ void __launch_bounds__(kRowMaxBlock) dequant_kernel(const DequantPara
         const uint32_t w = i < 4 ? u[k].x : u[k].y;
         f[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * (i & 3)))) * s;
       }
-      store8<VEC, BF16>(y, j0 + k, t, group, p.D, f);
+      store8<CUT>(y, j0 + k, t, group, sh, p.D, pack8<BF16>(f));
     }
   }
 }
@@ -303,10 +433,12 @@ __global__ void __launch_bounds__(kRowMaxBlock) dequant_kernel(const DequantPara
 namespace {
 
 // Threads of a row and 8-element chunks a thread: the smallest power of two that leaves at
-// most four chunks a thread (eight in rows of more than 16,384 elements); with few rows, more threads a row (down to one chunk each), since
-// the chip then waits on one row's loads and not on bandwidth.
-int row_group(int rows, int D, int num_sms, int* chunks) {
-  const int n = (D + 7) / 8;
+// most four chunks a thread (eight in rows of more than 16,384 elements); with few rows, more threads
+// a row (down to one chunk each), since the chip then waits on one row's loads and not on bandwidth.
+// Two chunks instead of four at many rows: 8192 x 4096 rmsnorm_i8 22.7 -> 31.1 us. `extra`: elements in
+// front of the row that its chunks cover too (kShifted).
+int row_group(int rows, int D, int extra, int num_sms, int* chunks) {
+  const int n = (D + extra + 7) / 8;
   int g = 16;
   while (g < kRowMaxBlock && (n + g - 1) / g > 4) g *= 2;
   while (rows <= 2 * num_sms && g < kRowMaxBlock && (n + g - 1) / g > 1) g *= 2;
@@ -314,24 +446,34 @@ int row_group(int rows, int D, int num_sms, int* chunks) {
   return g;
 }
 
-template <int MODE, bool BF16, int VEC>
+template <int MODE, bool BF16, int CUT>
 cudaError_t launch_rows(const RowParams& p, int chunks, cudaStream_t s) {
   const int block = p.group < kRowBlock ? kRowBlock : p.group;
   const int per = block / p.group;
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.rows) + per - 1) / per));
+  auto go = [&](auto kern, int v) {
+    const size_t smem = CUT == kShifted && MODE != kRowNorm ? size_t(per) * (v * p.group + 1) * 8 : 0;
+    return launch_ex(kern, grid, dim3(block), smem, s, true, 1, p);
+  };
   switch (chunks) {
-    case 1: return launch_ex(row_kernel<MODE, BF16, 1, VEC>, grid, dim3(block), 0, s, true, 1, p);
-    case 2: return launch_ex(row_kernel<MODE, BF16, 2, VEC>, grid, dim3(block), 0, s, true, 1, p);
-    case 3: return launch_ex(row_kernel<MODE, BF16, 3, VEC>, grid, dim3(block), 0, s, true, 1, p);
-    case 4: return launch_ex(row_kernel<MODE, BF16, 4, VEC>, grid, dim3(block), 0, s, true, 1, p);
-    default: return launch_ex(row_kernel<MODE, BF16, 8, VEC>, grid, dim3(block), 0, s, true, 1, p);
+    case 1: return go(row_kernel<MODE, BF16, 1, CUT>, 1);
+    case 2: return go(row_kernel<MODE, BF16, 2, CUT>, 2);
+    case 3: return go(row_kernel<MODE, BF16, 3, CUT>, 3);
+    case 4: return go(row_kernel<MODE, BF16, 4, CUT>, 4);
+    default: return go(row_kernel<MODE, BF16, 9, CUT>, 9);  // 9: 32,768 elements behind a shift
   }
 }
 
 template <int MODE>
-cudaError_t launch_mode(const RowParams& p, bool bf16, bool wide, int chunks, cudaStream_t s) {
-  if (bf16) return wide ? launch_rows<MODE, true, 8>(p, chunks, s) : launch_rows<MODE, true, 1>(p, chunks, s);
-  return wide ? launch_rows<MODE, false, 8>(p, chunks, s) : launch_rows<MODE, false, 1>(p, chunks, s);
+cudaError_t launch_mode(const RowParams& p, bool bf16, Cut cut, int chunks, cudaStream_t s) {
+  switch (cut) {
+    case kAligned:
+      return bf16 ? launch_rows<MODE, true, kAligned>(p, chunks, s) : launch_rows<MODE, false, kAligned>(p, chunks, s);
+    case kShifted:
+      return bf16 ? launch_rows<MODE, true, kShifted>(p, chunks, s) : launch_rows<MODE, false, kShifted>(p, chunks, s);
+    default:
+      return bf16 ? launch_rows<MODE, true, kSingle>(p, chunks, s) : launch_rows<MODE, false, kSingle>(p, chunks, s);
+  }
 }
 
 bool off(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
@@ -381,16 +523,28 @@ int run_rows(const char* who, int mode, RowParams p, int dtype, void* stream) {
   int dev = 0, sms = 0;
   rc = unit_device(&dev, &sms);
   if (rc) return rc;
-  const bool wide = p.D % 8 == 0 && !off(p.x, 16) && !off(p.residual, 16) && !off(p.weight, 16) && !off(p.sum, 16) &&
-                    !off(p.y, 16) && !off(p.q, 8) && p.ldx % 8 == 0 && (!p.residual || p.ldr % 8 == 0) &&
-                    (!p.sum || p.lds % 8 == 0) && (i8 ? p.ldq % 8 == 0 : p.ldy % 8 == 0);
+  // the cut that the operands allow (see Cut)
+  bool aligned = p.D % 8 == 0, shifted = !off(p.weight, 16) && (!i8 || (!off(p.q, 8) && p.ldq % 8 == 0));
+  auto look = [&](const uint16_t* q, int64_t ld) {
+    if (!q) return;
+    aligned = aligned && !off(q, 16) && ld % 8 == 0;
+    shifted = shifted && ((reinterpret_cast<uintptr_t>(q) ^ reinterpret_cast<uintptr_t>(p.x)) & 15) == 0 &&
+              (p.rows == 1 || (ld - p.ldx) % 8 == 0);
+  };
+  look(p.x, p.ldx);
+  look(p.residual, p.ldr);
+  look(p.sum, p.lds);
+  look(p.y, p.ldy);
+  aligned = aligned && shifted;
+  const Cut cut = aligned ? kAligned : shifted ? kShifted : kSingle;
   int chunks = 0;
-  p.group = row_group(p.rows, p.D, sms, &chunks);
+  p.group = row_group(p.rows, p.D, cut == kShifted ? 7 : 0, sms, &chunks);
+  p.inv_D = 1.0f / static_cast<float>(p.D);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == BBH_BF16;
-  const cudaError_t e = mode == kRowNorm     ? launch_mode<kRowNorm>(p, bf, wide, chunks, s)
-                        : mode == kRowNormI8 ? launch_mode<kRowNormI8>(p, bf, wide, chunks, s)
-                                             : launch_mode<kRowQuant>(p, bf, wide, chunks, s);
+  const cudaError_t e = mode == kRowNorm     ? launch_mode<kRowNorm>(p, bf, cut, chunks, s)
+                        : mode == kRowNormI8 ? launch_mode<kRowNormI8>(p, bf, cut, chunks, s)
+                                             : launch_mode<kRowQuant>(p, bf, cut, chunks, s);
   if (e != cudaSuccess) return internal_fail(BBH_ERR_CUDA, w + ": " + cudaGetErrorString(e));
   return BBH_OK;
 }
@@ -403,20 +557,20 @@ extern "C" {
 int bbh_rmsnorm(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr, const uint16_t* weight,
                 uint16_t* y, int64_t ldy, uint16_t* sum, int64_t lds, int M, int D, float eps, int dtype,
                 void* stream) {
-  bbh::RowParams p{x, residual, weight, y, nullptr, nullptr, sum, ldx, ldr, ldy, 0, lds, M, D, 0, eps};
+  bbh::RowParams p{x, residual, weight, y, nullptr, nullptr, sum, ldx, ldr, ldy, 0, lds, M, D, 0, eps, 0.f};
   return bbh::run_rows("bbh_rmsnorm", bbh::kRowNorm, p, dtype, stream);
 }
 
 int bbh_rmsnorm_i8(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr, const uint16_t* weight,
                    int8_t* q, int64_t ldq, float* scale, uint16_t* sum, int64_t lds, int M, int D, float eps,
                    int dtype, void* stream) {
-  bbh::RowParams p{x, residual, weight, nullptr, q, scale, sum, ldx, ldr, 0, ldq, lds, M, D, 0, eps};
+  bbh::RowParams p{x, residual, weight, nullptr, q, scale, sum, ldx, ldr, 0, ldq, lds, M, D, 0, eps, 0.f};
   return bbh::run_rows("bbh_rmsnorm_i8", bbh::kRowNormI8, p, dtype, stream);
 }
 
 int bbh_quantize_i8(const uint16_t* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int M, int D, int dtype,
                     void* stream) {
-  bbh::RowParams p{x, nullptr, nullptr, nullptr, q, scale, nullptr, ldx, 0, 0, ldq, 0, M, D, 0, 0.f};
+  bbh::RowParams p{x, nullptr, nullptr, nullptr, q, scale, nullptr, ldx, 0, 0, ldq, 0, M, D, 0, 0.f, 0.f};
   return bbh::run_rows("bbh_quantize_i8", bbh::kRowQuant, p, dtype, stream);
 }
 
@@ -436,17 +590,19 @@ int bbh_dequantize_i8(const int8_t* q, int64_t ldq, const float* scale, uint16_t
   int dev = 0, sms = 0;
   rc = unit_device(&dev, &sms);
   if (rc) return rc;
-  const bool wide = D % 8 == 0 && !off(q, 8) && !off(y, 16) && ldq % 8 == 0 && ldy % 8 == 0;
+  const bool q8 = !off(q, 8) && ldq % 8 == 0;
+  const Cut cut = q8 && D % 8 == 0 && !off(y, 16) && ldy % 8 == 0 ? kAligned : q8 ? kShifted : kSingle;
   int chunks = 0;
-  DequantParams p{q, scale, y, ldq, ldy, M, D, row_group(M, D, sms, &chunks)};
+  DequantParams p{q, scale, y, ldq, ldy, M, D, row_group(M, D, cut == kShifted ? 7 : 0, sms, &chunks)};
   const int block = p.group < kRowBlock ? kRowBlock : p.group;
   const int per = block / p.group;
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(M) + per - 1) / per));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kern) { return launch_ex(kern, grid, dim3(block), 0, s, true, 1, p); };
   const bool bf = dtype == BBH_BF16;
-  auto kern = bf ? (wide ? dequant_kernel<true, 8> : dequant_kernel<true, 1>)
-                 : (wide ? dequant_kernel<false, 8> : dequant_kernel<false, 1>);
-  const cudaError_t e = launch_ex(kern, grid, dim3(block), 0, s, true, 1, p);
+  const cudaError_t e = cut == kAligned   ? (bf ? go(dequant_kernel<true, kAligned>) : go(dequant_kernel<false, kAligned>))
+                        : cut == kShifted ? (bf ? go(dequant_kernel<true, kShifted>) : go(dequant_kernel<false, kShifted>))
+                                          : (bf ? go(dequant_kernel<true, kSingle>) : go(dequant_kernel<false, kSingle>));
   if (e != cudaSuccess)
     return internal_fail(BBH_ERR_CUDA, std::string("bbh_dequantize_i8: ") + cudaGetErrorString(e));
   return BBH_OK;

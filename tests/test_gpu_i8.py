@@ -136,6 +136,48 @@ def test_row_strides_and_alignments(M, D, ld, offset, dtype):
         assert bool((buf == 7.0).all())
 
 
+@pytest.mark.parametrize("D", [5, 8, 63, 384, 1023, 4095, 16381, 32761])
+def test_every_alignment_of_a_row(D):
+    """Rows that start 0 to 7 elements behind a 16-byte boundary, alone and as the rows of one call of odd
+    width, and a weight at an odd address. Sums (not the order of the mean's terms), integers and what is
+    read back are the bits of the same rows elsewhere."""
+    import bbh
+
+    f16 = torch.float16
+    g = gen("align", D)
+    x, r = rows16(16, D, f16, g), rows16(16, D, f16, g)
+    w = torch.randn(D, generator=g, device=DEV).half()
+    t = x.double() + r.double()
+    want = t / (t.square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+    want_s = want.abs().amax(1) / 127
+    y, v = bbh.rmsnorm(x, w, residual=r)
+    assert_close16(y, want, 50, f16)
+    q, s, _ = bbh.rmsnorm_i8(x, w, residual=r)
+    check_quantized(q, s, want, 6, 55)
+    q2, s2 = bbh.quantize_i8(x)
+    z = bbh.dequantize_i8(q2, s2)
+    for off in range(8):
+        one = lambda t, i: torch.cat([t.new_empty(off), t[i]])[off:].view(1, D)
+        i = (3 * off + 1) % 16
+        xo, ro = one(x, i), one(r, i)
+        assert (xo.data_ptr() // 2) % 8 == off
+        out, so = one(y, 0), one(y, 0)
+        bbh.rmsnorm(xo, w, residual=ro, out=out, sum_out=so)
+        assert_close16(out[0], want[i], 50, f16)
+        assert torch.equal(so[0], v[i])
+        a, b, c = bbh.rmsnorm_i8(xo, w, residual=ro, sum_out=so)
+        assert torch.equal(a[0], q[i]) and torch.equal(c[0], v[i])
+        assert abs(b[0].double() - want_s[i]) <= 55 * U * want_s[i]
+        a, b = bbh.quantize_i8(xo)
+        assert torch.equal(a[0], q2[i]) and b[0] == s2[i]
+        bbh.dequantize_i8(a, b, out=out)
+        assert torch.equal(out[0], z[i])
+    w1 = torch.cat([w[:1], w])[1:]
+    assert_close16(bbh.rmsnorm(x, w1, residual=r)[0], want, 50, f16)
+    a, b, _ = bbh.rmsnorm_i8(x, w1, residual=r)
+    assert torch.equal(a, q) and bool(((b.double() - want_s).abs() <= 55 * U * want_s).all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("M,D", SHAPES)
