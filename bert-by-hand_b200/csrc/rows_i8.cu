@@ -183,14 +183,22 @@ __device__ __forceinline__ uint2 low_bytes(const uint32_t* b) {
                     __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
+// 127 / top from the hardware's reciprocal (off by 2^-23 at most) and 3 * 2^-23 more, so that with its two
+// roundings it is above 127 / top by 0 to 5 * 2^-23 of it.
+__device__ __forceinline__ float steps_per_unit(float top) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
+  return r * 127.f * (1.f + 3 * 0x1p-23f);
+}
+
 // rint(f * 127 / top) of eight values as bytes: the low byte of f * inv + 1.5 * 2^23, one fma that
-// rounds half to even. inv is 127 / top rounded up; f * inv <= 127 (1 + 2^-22), which rounds to 127.
+// rounds half to even, with inv from steps_per_unit; f * inv < 127.0001 rounds to 127.
 //
-// Elements of a 16-bit row (kRowQuant) meet exact halves, which a rounded inv would push to either
-// side. If 127 does not divide top's significand the only one is |f| = top / 2, 63.5 steps, and inv rounded
-// up takes it to 64, the even neighbour (other values are 2^-20 of themselves or more away from a
-// half). If 127 divides it (`ties`), f * inv + f * rest, with rest what inv lacks of 127 / top, is right
-// to fp32 and a half stays one.
+// Elements of a 16-bit row (kRowQuant) meet exact halves, which an inexact inv pushes to either side.
+// If 127 does not divide top's significand the only one is |f| = top / 2, 63.5 steps, and inv, being
+// above, takes it to 64, the even neighbour; with 11-bit significands every other value is at least
+// 2^-20 of itself away from a half, more than inv is off. If 127 divides it (`ties`), f * inv + f * rest,
+// with rest what inv lacks of 127 / top, is right to fp32 and a half stays one.
 __device__ __forceinline__ uint2 quantize8(const float* f, float inv, float rest, bool ties) {
   uint32_t b[8];
   if (ties) {
@@ -254,18 +262,18 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
   }
 
   float f[8 * V];
-  float ss = 0.f, top = 0.f;
+  float ss = 0.f, ss1 = 0.f, top = 0.f;
   uint32_t top2 = 0;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     float* v = f + 8 * j;
-    unpack8<BF16>(ux[j], v);
-    if constexpr (MODE == kRowQuant) {
+    if constexpr (MODE == kRowQuant) {  // the packed values are enough until the scale is known
       top2 = max_abs_nan2<BF16>(top2, ux[j].x);
       top2 = max_abs_nan2<BF16>(top2, ux[j].y);
       top2 = max_abs_nan2<BF16>(top2, ux[j].z);
       top2 = max_abs_nan2<BF16>(top2, ux[j].w);
     } else {
+      unpack8<BF16>(ux[j], v);
       if (p.residual) {
         float u[8];
         unpack8<BF16>(ur[j], u);
@@ -274,7 +282,10 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
         if (p.sum) store8<CUT>(p.sum + r * p.lds, j, t, group, sh, D, pack8<BF16>(v));
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+      for (int i = 0; i < 8; i += 2) {
+        ss = fmaf(v[i], v[i], ss);
+        ss1 = fmaf(v[i + 1], v[i + 1], ss1);
+      }
     }
     if constexpr (MODE == kRowNormI8) {
       if (p.weight) {
@@ -291,6 +302,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     const float2 m = unpack16<BF16>(top2);
     top = max_nan(m.x, m.y);
   }
+  ss += ss1;
   group_reduce<MODE != kRowQuant, MODE != kRowNorm>(ss, top, group);
   const float rstd = MODE == kRowQuant ? 1.f : rsqrtf(ss * p.inv_D + p.eps);
 
@@ -314,7 +326,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     // that whatever is computed from it is NaN too.
     const bool finite = top <= FLT_MAX;
     const bool zero = !finite || top < 0x1p-120f;
-    const float inv = __fdiv_ru(127.f, zero ? 1.f : top);
+    const float inv = steps_per_unit(zero ? 1.f : top);
     bool ties = false;
     float rest = 0.f;
     if constexpr (MODE == kRowQuant) {
@@ -329,7 +341,10 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
       extern __shared__ uint2 s_q[];
       uint2* row = s_q + (threadIdx.x / group) * (V * group + 1);
 #pragma unroll
-      for (int j = 0; j < V; ++j) row[j * group + t] = quantize8(f + 8 * j, inv, rest, ties);
+      for (int j = 0; j < V; ++j) {
+        if (MODE == kRowQuant) unpack8<BF16>(ux[j], f + 8 * j);
+        row[j * group + t] = quantize8(f + 8 * j, inv, rest, ties);
+      }
       if (t == 0) row[V * group] = make_uint2(0, 0);
       __syncthreads();
       for (int c = t; 8 * c < D; c += group) {  // elements 8c ..: bytes sh .. of chunk c, then of chunk c + 1
@@ -346,6 +361,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
+        if (MODE == kRowQuant) unpack8<BF16>(ux[j], f + 8 * j);
         uint2 o = quantize8(f + 8 * j, inv, rest, ties);
         if (zero) o = make_uint2(0, 0);
         const int e = elem<CUT>(j, 0, t, group, 0);
