@@ -77,88 +77,116 @@ __device__ __forceinline__ uint32_t max_abs_nan2(uint32_t m, uint32_t w) {
   return d;
 }
 
-// How a row is cut into the 8-element chunks of its threads; chunk c = j * group + t is thread t's j-th.
+// How a row is cut for its threads, 8 elements a chunk; chunk c = j * group + t is thread t's j-th.
 //  kAligned  chunk c is elements 8c .. 8c + 7, one 16-byte access: rows 16-byte aligned, D a multiple of 8.
-//  kShifted  the 16-bit tensors' rows start `sh` elements behind a 16-byte boundary, the same for all of
-//            them (contiguous tensors of any width are so): chunk c is elements 8c - sh .. 8c - sh + 7, which
-//            is one 16-byte access inside the row; the row's first and last chunk go element by element.
+//  kShifted  the 16-bit tensors' rows start anywhere, but all of them at the same distance from a 16-byte
+//            boundary (contiguous tensors of any width do): chunk c is elements head + 8c .., one 16-byte
+//            access; the `head` elements in front of the first chunk and the rest behind the last one go
+//            to one thread each.
 //  kSingle   any strides and alignments: elements `group` apart, 2-byte accesses.
 enum Cut : int { kAligned, kShifted, kSingle };
 
-template <int CUT>
-__device__ __forceinline__ int elem(int j, int i, int t, int group, int sh) {
-  if (CUT == kSingle) return (8 * j + i) * group + t;
-  return 8 * (j * group + t) + i - (CUT == kShifted ? sh : 0);
-}
+// A thread's place in its row.
+struct Place {
+  int t, group, D;
+  int head;    // elements in front of the first chunk (0 but for kShifted)
+  int chunks;  // whole chunks (kAligned, kShifted)
+  int edge;    // this thread's element outside the chunks, or -1 (kShifted)
+};
 
-// Elements e .. e + 7 one by one, zeros outside [0, D).
-__device__ __forceinline__ uint4 load_edge(const uint16_t* row, int e, int D) {
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (e + 8 > 0 && e < D) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (e + i >= 0 && e + i < D) w[i >> 1] |= static_cast<uint32_t>(row[e + i]) << (16 * (i & 1));
+template <int CUT>
+__device__ __forceinline__ Place place(const uint16_t* row, int t, int group, int D) {
+  Place p{t, group, D, 0, D / 8, -1};
+  if constexpr (CUT == kShifted) {
+    p.head = min(D, static_cast<int>(-(reinterpret_cast<uintptr_t>(row) >> 1) & 7));
+    p.chunks = (D - p.head) / 8;
+    const int tail = p.head + 8 * p.chunks;
+    if (t < 8) {
+      if (t < p.head) p.edge = t;
+    } else if (t < 16 && tail + t - 8 < D) {
+      p.edge = tail + t - 8;
+    }
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return p;
 }
 
+// First element of the thread's j-th chunk, or -1.
 template <int CUT>
-__device__ __forceinline__ uint4 load8(const uint16_t* row, int j, int t, int group, int sh, int D) {
-  const int e = elem<CUT>(j, 0, t, group, sh);
-  if constexpr (CUT == kAligned) {
-    return e < D ? *reinterpret_cast<const uint4*>(row + e) : make_uint4(0, 0, 0, 0);
-  } else if constexpr (CUT == kShifted) {
-    return e >= 0 && e + 8 <= D ? *reinterpret_cast<const uint4*>(row + e) : load_edge(row, e, D);
-  } else {
+__device__ __forceinline__ int chunk_at(const Place& p, int j) {
+  const int c = j * p.group + p.t;
+  return c < p.chunks ? p.head + 8 * c : -1;
+}
+// Element i of chunk j, kSingle.
+__device__ __forceinline__ int single_at(const Place& p, int j, int i) { return (8 * j + i) * p.group + p.t; }
+
+template <int CUT>
+__device__ __forceinline__ uint4 load8(const uint16_t* row, const Place& p, int j) {
+  if constexpr (CUT == kSingle) {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = elem<kSingle>(j, i, t, group, 0);
-      if (k < D) w[i >> 1] |= static_cast<uint32_t>(row[k]) << (16 * (i & 1));
-    }
+    for (int i = 0; i < 8; ++i)
+      if (single_at(p, j, i) < p.D) w[i >> 1] |= static_cast<uint32_t>(row[single_at(p, j, i)]) << (16 * (i & 1));
     return make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    const int e = chunk_at<CUT>(p, j);
+    return e >= 0 ? *reinterpret_cast<const uint4*>(row + e) : make_uint4(0, 0, 0, 0);
   }
 }
 
 template <int CUT>
-__device__ __forceinline__ void store8(uint16_t* row, int j, int t, int group, int sh, int D, uint4 u) {
-  const int e = elem<CUT>(j, 0, t, group, sh);
-  if (CUT == kAligned) {
-    if (e < D) *reinterpret_cast<uint4*>(row + e) = u;
-    return;
-  }
-  if (CUT == kShifted && e >= 0 && e + 8 <= D) {
-    *reinterpret_cast<uint4*>(row + e) = u;
-    return;
-  }
-  if (CUT == kSingle || (e + 8 > 0 && e < D)) {
+__device__ __forceinline__ void store8(uint16_t* row, const Place& p, int j, uint4 u) {
+  if constexpr (CUT == kSingle) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int k = elem<CUT>(j, i, t, group, sh);
-      if (k >= 0 && k < D) row[k] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
-    }
+    for (int i = 0; i < 8; ++i)
+      if (single_at(p, j, i) < p.D) row[single_at(p, j, i)] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+  } else {
+    const int e = chunk_at<CUT>(p, j);
+    if (e >= 0) *reinterpret_cast<uint4*>(row + e) = u;
   }
 }
 
-// A chunk of the weight, whose start is 16-byte aligned where the rows' is not (kShifted): the eight
-// elements lie in two neighbouring 16-byte pieces, taken out of their eight words by `sh`.
+// A chunk of the weight, which is 16-byte aligned where the rows may not be (kShifted): elements e .. e + 7
+// lie in two neighbouring 16-byte pieces and are taken out of their eight words.
 template <int CUT>
-__device__ __forceinline__ uint4 load_weight8(const uint16_t* weight, int j, int t, int group, int sh, int D) {
-  if (CUT != kShifted || sh == 0) return load8<CUT>(weight, j, t, group, sh, D);
-  const int c = j * group + t;  // elements 8c - sh ..: the end of piece c - 1, the start of piece c
-  if (c == 0 || 8 * c + 8 > D) return load_edge(weight, 8 * c - sh, D);
-  const uint4 lo = *reinterpret_cast<const uint4*>(weight + 8 * c - 8);
-  const uint4 hi = *reinterpret_cast<const uint4*>(weight + 8 * c);
+__device__ __forceinline__ uint4 load_weight8(const uint16_t* weight, const Place& p, int j) {
+  if (CUT != kShifted || (p.head & 7) == 0) return load8<CUT>(weight, p, j);
+  const int e = chunk_at<CUT>(p, j);
+  if (e < 0) return make_uint4(0, 0, 0, 0);
+  const int base = e - p.head;  // a multiple of 8
+  const uint4 lo = *reinterpret_cast<const uint4*>(weight + base);
+  uint4 hi;
+  if (base + 16 <= p.D) {
+    hi = *reinterpret_cast<const uint4*>(weight + base + 8);
+  } else {  // the piece ends behind the weight
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = 0; i < p.head; ++i) {
+      const uint32_t b = static_cast<uint32_t>(weight[base + 8 + i]) << (16 * (i & 1));
+      w[0] |= i < 2 ? b : 0u;
+      w[1] |= i >> 1 == 1 ? b : 0u;
+      w[2] |= i >> 1 == 2 ? b : 0u;
+      w[3] |= i >> 1 == 3 ? b : 0u;
+    }
+    hi = make_uint4(w[0], w[1], w[2], w[3]);
+  }
   uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-  const int words = (8 - sh) >> 1;  // 0 .. 3
+  const int words = p.head >> 1;  // 0 .. 3
 #pragma unroll
   for (int i = 0; i < 6; ++i) w[i] = words & 2 ? w[i + 2] : w[i];
 #pragma unroll
   for (int i = 0; i < 5; ++i) w[i] = words & 1 ? w[i + 1] : w[i];
-  const uint32_t pick = sh & 1 ? 0x5432u : 0x3210u;
+  const uint32_t pick = p.head & 1 ? 0x5432u : 0x3210u;
   return make_uint4(__byte_perm(w[0], w[1], pick), __byte_perm(w[1], w[2], pick), __byte_perm(w[2], w[3], pick),
                     __byte_perm(w[3], w[4], pick));
+}
+
+template <bool BF16>
+__device__ __forceinline__ float load1(const uint16_t* row, int e) {
+  return unpack16<BF16>(row[e]).x;
+}
+template <bool BF16>
+__device__ __forceinline__ void store1(uint16_t* row, int e, float f) {
+  row[e] = static_cast<uint16_t>(pack16<BF16>(f, 0.f));
 }
 
 template <bool BF16>
@@ -210,6 +238,9 @@ __device__ __forceinline__ uint2 quantize8(const float* f, float inv, float rest
   }
   return low_bytes(b);
 }
+__device__ __forceinline__ uint8_t quantize1(float f, float inv, float rest, bool ties) {
+  return static_cast<uint8_t>(__float_as_uint(ties ? fmaf(f, inv, f * rest) + 12582912.f : fmaf(f, inv, 12582912.f)));
+}
 
 // Sum of s and maximum of m over the `group` threads of a row (a power of two from 16 on; groups of
 // more than a warp exchange through shared memory). Every thread of the block calls it.
@@ -248,17 +279,25 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
   const int t = threadIdx.x & (group - 1);
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
   const bool live = r < p.rows;
-  const int D = live ? p.D : 0;  // a group behind the last row loads and stores nothing
   const uint16_t* x = p.x + r * p.ldx;
-  const int sh = CUT == kShifted ? static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15) >> 1 : 0;
+  const uint16_t* residual = MODE != kRowQuant && p.residual ? p.residual + r * p.ldr : nullptr;
+  const uint16_t* weight = MODE != kRowQuant ? p.weight : nullptr;
+  uint16_t* sum = p.sum + r * p.lds;
+  const Place at = place<CUT>(x, t, group, live ? p.D : 0);  // a group behind the last row has no elements
+  const bool edge = CUT == kShifted && at.edge >= 0;
   pdl_wait();
 
   uint4 ux[V], ur[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) ux[j] = load8<CUT>(x, j, t, group, sh, D);
-  if (MODE != kRowQuant && p.residual) {
+  for (int j = 0; j < V; ++j) ux[j] = load8<CUT>(x, at, j);
+  if (residual) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) ur[j] = load8<CUT>(p.residual + r * p.ldr, j, t, group, sh, D);
+    for (int j = 0; j < V; ++j) ur[j] = load8<CUT>(residual, at, j);
+  }
+  float fe = 0.f;  // the edge element
+  if (edge) {
+    fe = load1<BF16>(x, at.edge);
+    if (residual) fe += load1<BF16>(residual, at.edge);
   }
 
   float f[8 * V];
@@ -274,12 +313,12 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
       top2 = max_abs_nan2<BF16>(top2, ux[j].w);
     } else {
       unpack8<BF16>(ux[j], v);
-      if (p.residual) {
+      if (residual) {
         float u[8];
         unpack8<BF16>(ur[j], u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += u[i];
-        if (p.sum) store8<CUT>(p.sum + r * p.lds, j, t, group, sh, D, pack8<BF16>(v));
+        if (p.sum) store8<CUT>(sum, at, j, pack8<BF16>(v));
       }
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
@@ -288,9 +327,9 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
       }
     }
     if constexpr (MODE == kRowNormI8) {
-      if (p.weight) {
+      if (weight) {
         float u[8];
-        unpack8<BF16>(load_weight8<CUT>(p.weight, j, t, group, sh, D), u);
+        unpack8<BF16>(load_weight8<CUT>(weight, at, j), u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= u[i];
       }
@@ -302,24 +341,32 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     const float2 m = unpack16<BF16>(top2);
     top = max_nan(m.x, m.y);
   }
+  if (edge) {
+    if (residual && p.sum) store1<BF16>(sum, at.edge, fe);
+    ss1 = fmaf(fe, fe, ss1);
+    if (weight) fe *= load1<BF16>(weight, at.edge);
+    top = max_abs_nan(top, fe, 0.f);
+  }
   ss += ss1;
   group_reduce<MODE != kRowQuant, MODE != kRowNorm>(ss, top, group);
   const float rstd = MODE == kRowQuant ? 1.f : rsqrtf(ss * p.inv_D + p.eps);
 
   if constexpr (MODE == kRowNorm) {
+    uint16_t* y = p.y + r * p.ldy;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float* v = f + 8 * j;
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= rstd;
-      if (p.weight) {
+      if (weight) {
         float u[8];
-        unpack8<BF16>(load_weight8<CUT>(p.weight, j, t, group, sh, D), u);
+        unpack8<BF16>(load_weight8<CUT>(weight, at, j), u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= u[i];
       }
-      store8<CUT>(p.y + r * p.ldy, j, t, group, sh, D, pack8<BF16>(v));
+      store8<CUT>(y, at, j, pack8<BF16>(v));
     }
+    if (edge) store1<BF16>(y, at.edge, fe * rstd);
   } else {
     // A row whose largest magnitude is below 2^-120 (127 / top would near the end of fp32) is
     // stored as zeros with scale 0; one with a NaN or an infinity as zeros with scale NaN, so
@@ -336,26 +383,27 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     if (live && t == 0) p.scale[r] = finite ? (zero ? 0.f : top / 127.f) * rstd : __int_as_float(0x7fc00000);
     int8_t* q = p.q + r * p.ldq;
     if constexpr (CUT == kShifted) {
-      // The bytes of a chunk are not where an aligned store of q wants them: through shared memory. The
-      // rows of q are 8-byte aligned.
+      // The bytes of a chunk are not where an aligned store of q wants them: through shared memory, element e
+      // at byte e + sh, so that chunks are 8-byte pieces there. The rows of q are 8-byte aligned.
       extern __shared__ uint2 s_q[];
-      uint2* row = s_q + (threadIdx.x / group) * (V * group + 1);
+      uint2* row = s_q + (threadIdx.x / group) * (V * group + 2);
+      const int sh = -at.head & 7, first = sh ? 1 : 0;  // the piece of chunk 0
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if (MODE == kRowQuant) unpack8<BF16>(ux[j], f + 8 * j);
-        row[j * group + t] = quantize8(f + 8 * j, inv, rest, ties);
+        if (chunk_at<CUT>(at, j) >= 0) row[first + j * group + t] = quantize8(f + 8 * j, inv, rest, ties);
       }
-      if (t == 0) row[V * group] = make_uint2(0, 0);
+      if (edge) reinterpret_cast<uint8_t*>(row)[at.edge + sh] = quantize1(fe, inv, rest, ties);
       __syncthreads();
-      for (int c = t; 8 * c < D; c += group) {  // elements 8c ..: bytes sh .. of chunk c, then of chunk c + 1
+      for (int c = t; 8 * c < at.D; c += group) {  // elements 8c ..: bytes sh .. of piece c, then of piece c + 1
         const uint2 a = row[c], b = row[c + 1];
         const uint64_t lo = static_cast<uint64_t>(a.y) << 32 | a.x, hi = static_cast<uint64_t>(b.y) << 32 | b.x;
         uint64_t o = sh ? lo >> (8 * sh) | hi << (64 - 8 * sh) : lo;
         if (zero) o = 0;
-        if (8 * c + 8 <= D) {
+        if (8 * c + 8 <= at.D) {
           *reinterpret_cast<uint64_t*>(q + 8 * c) = o;
         } else {
-          for (int i = 0; 8 * c + i < D; ++i) q[8 * c + i] = static_cast<int8_t>(o >> (8 * i));
+          for (int i = 0; 8 * c + i < at.D; ++i) q[8 * c + i] = static_cast<int8_t>(o >> (8 * i));
         }
       }
     } else {
@@ -364,15 +412,14 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
         if (MODE == kRowQuant) unpack8<BF16>(ux[j], f + 8 * j);
         uint2 o = quantize8(f + 8 * j, inv, rest, ties);
         if (zero) o = make_uint2(0, 0);
-        const int e = elem<CUT>(j, 0, t, group, 0);
         if constexpr (CUT == kAligned) {
-          if (e < D) *reinterpret_cast<uint2*>(q + e) = o;
+          const int e = chunk_at<CUT>(at, j);
+          if (e >= 0) *reinterpret_cast<uint2*>(q + e) = o;
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int k = elem<kSingle>(j, i, t, group, 0);
-            if (k < D) q[k] = static_cast<int8_t>((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
-          }
+          for (int i = 0; i < 8; ++i)
+            if (single_at(at, j, i) < at.D)
+              q[single_at(at, j, i)] = static_cast<int8_t>((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
         }
       }
     }
@@ -388,16 +435,19 @@ struct DequantParams {
   int rows, D, group;
 };
 
-// Eight bytes of q from element e on, where q + e is `sh` bytes before an 8-byte boundary.
-__device__ __forceinline__ uint2 load_q8(const int8_t* q, int e, int sh, int D) {
-  uint64_t o = 0;
-  if (e >= 0 && e + sh + 8 <= D) {
-    const uint64_t hi = *reinterpret_cast<const uint64_t*>(q + e + sh);
-    o = sh ? *reinterpret_cast<const uint64_t*>(q + e + sh - 8) >> (64 - 8 * sh) | hi << (8 * sh) : hi;
-  } else {
-    for (int i = 0; i < 8; ++i)
-      if (e + i >= 0 && e + i < D) o |= static_cast<uint64_t>(static_cast<uint8_t>(q[e + i])) << (8 * i);
+// Eight bytes of q, whose rows are 8-byte aligned, from element e = base + head on (base a multiple of 8).
+__device__ __forceinline__ uint2 load_q8(const int8_t* q, int e, int head, int D) {
+  const int base = e - head;
+  const uint64_t lo = *reinterpret_cast<const uint64_t*>(q + base);
+  uint64_t hi = 0;
+  if (head) {
+    if (base + 16 <= D) {
+      hi = *reinterpret_cast<const uint64_t*>(q + base + 8);
+    } else {
+      for (int i = 0; i < head; ++i) hi |= static_cast<uint64_t>(static_cast<uint8_t>(q[base + 8 + i])) << (8 * i);
+    }
   }
+  const uint64_t o = head ? lo >> (8 * head) | hi << (64 - 8 * head) : lo;
   return make_uint2(static_cast<uint32_t>(o), static_cast<uint32_t>(o >> 32));
 }
 
@@ -405,32 +455,29 @@ template <bool BF16, int CUT>
 __global__ void __launch_bounds__(kRowMaxBlock) dequant_kernel(const DequantParams p) {
   pdl_launch_dependents();
   const int group = p.group;
-  const int t = threadIdx.x & (group - 1);
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
   pdl_wait();
   if (r >= p.rows) return;
   const int8_t* q = p.q + r * p.ldq;
   uint16_t* y = p.y + r * p.ldy;
-  const int sh = CUT == kShifted ? static_cast<int>(reinterpret_cast<uintptr_t>(y) & 15) >> 1 : 0;
+  const Place at = place<CUT>(y, threadIdx.x & (group - 1), group, p.D);
   const float s = p.scale[r];
-  for (int j0 = 0; elem<CUT>(j0, 0, t, group, sh) < p.D; j0 += 4) {
+  const int chunks = CUT == kSingle ? (p.D + 7) / 8 : at.chunks;
+  for (int j0 = 0; j0 * group < chunks; j0 += 4) {
     uint2 u[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int e = elem<CUT>(j0 + k, 0, t, group, sh);
       u[k] = make_uint2(0, 0);
-      if constexpr (CUT == kAligned) {
-        if (e < p.D) u[k] = *reinterpret_cast<const uint2*>(q + e);
-      } else if constexpr (CUT == kShifted) {
-        if (e < p.D) u[k] = load_q8(q, e, sh, p.D);
-      } else {
+      if constexpr (CUT == kSingle) {
         uint32_t w[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int m = elem<kSingle>(j0 + k, i, t, group, 0);
-          if (m < p.D) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(q[m])) << (8 * (i & 3));
-        }
+        for (int i = 0; i < 8; ++i)
+          if (single_at(at, j0 + k, i) < p.D)
+            w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(q[single_at(at, j0 + k, i)])) << (8 * (i & 3));
         u[k] = make_uint2(w[0], w[1]);
+      } else {
+        const int e = chunk_at<CUT>(at, j0 + k);
+        if (e >= 0) u[k] = load_q8(q, e, CUT == kShifted ? at.head : 0, p.D);
       }
     }
 #pragma unroll
@@ -441,9 +488,10 @@ __global__ void __launch_bounds__(kRowMaxBlock) dequant_kernel(const DequantPara
         const uint32_t w = i < 4 ? u[k].x : u[k].y;
         f[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * (i & 3)))) * s;
       }
-      store8<CUT>(y, j0 + k, t, group, sh, p.D, pack8<BF16>(f));
+      store8<CUT>(y, at, j0 + k, pack8<BF16>(f));
     }
   }
+  if (CUT == kShifted && at.edge >= 0) store1<BF16>(y, at.edge, static_cast<float>(q[at.edge]) * s);
 }
 
 namespace {
@@ -451,10 +499,9 @@ namespace {
 // Threads of a row and 8-element chunks a thread: the smallest power of two that leaves at
 // most four chunks a thread (eight in rows of more than 16,384 elements); with few rows, more threads
 // a row (down to one chunk each), since the chip then waits on one row's loads and not on bandwidth.
-// Two chunks instead of four at many rows: 8192 x 4096 rmsnorm_i8 22.7 -> 31.1 us. `extra`: elements in
-// front of the row that its chunks cover too (kShifted).
-int row_group(int rows, int D, int extra, int num_sms, int* chunks) {
-  const int n = (D + extra + 7) / 8;
+// Two chunks instead of four at many rows: 8192 x 4096 rmsnorm_i8 22.7 -> 31.1 us.
+int row_group(int rows, int D, int num_sms, int* chunks) {
+  const int n = (D + 7) / 8;
   int g = 16;
   while (g < kRowMaxBlock && (n + g - 1) / g > 4) g *= 2;
   while (rows <= 2 * num_sms && g < kRowMaxBlock && (n + g - 1) / g > 1) g *= 2;
@@ -468,7 +515,7 @@ cudaError_t launch_rows(const RowParams& p, int chunks, cudaStream_t s) {
   const int per = block / p.group;
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.rows) + per - 1) / per));
   auto go = [&](auto kern, int v) {
-    const size_t smem = CUT == kShifted && MODE != kRowNorm ? size_t(per) * (v * p.group + 1) * 8 : 0;
+    const size_t smem = CUT == kShifted && MODE != kRowNorm ? size_t(per) * (v * p.group + 2) * 8 : 0;
     return launch_ex(kern, grid, dim3(block), smem, s, true, 1, p);
   };
   switch (chunks) {
@@ -476,7 +523,7 @@ cudaError_t launch_rows(const RowParams& p, int chunks, cudaStream_t s) {
     case 2: return go(row_kernel<MODE, BF16, 2, CUT>, 2);
     case 3: return go(row_kernel<MODE, BF16, 3, CUT>, 3);
     case 4: return go(row_kernel<MODE, BF16, 4, CUT>, 4);
-    default: return go(row_kernel<MODE, BF16, 9, CUT>, 9);  // 9: 32,768 elements behind a shift
+    default: return go(row_kernel<MODE, BF16, 8, CUT>, 8);
   }
 }
 
@@ -554,7 +601,7 @@ int run_rows(const char* who, int mode, RowParams p, int dtype, void* stream) {
   aligned = aligned && shifted;
   const Cut cut = aligned ? kAligned : shifted ? kShifted : kSingle;
   int chunks = 0;
-  p.group = row_group(p.rows, p.D, cut == kShifted ? 7 : 0, sms, &chunks);
+  p.group = row_group(p.rows, p.D, sms, &chunks);
   p.inv_D = 1.0f / static_cast<float>(p.D);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == BBH_BF16;
@@ -609,7 +656,7 @@ int bbh_dequantize_i8(const int8_t* q, int64_t ldq, const float* scale, uint16_t
   const bool q8 = !off(q, 8) && ldq % 8 == 0;
   const Cut cut = q8 && D % 8 == 0 && !off(y, 16) && ldy % 8 == 0 ? kAligned : q8 ? kShifted : kSingle;
   int chunks = 0;
-  DequantParams p{q, scale, y, ldq, ldy, M, D, row_group(M, D, cut == kShifted ? 7 : 0, sms, &chunks)};
+  DequantParams p{q, scale, y, ldq, ldy, M, D, row_group(M, D, sms, &chunks)};
   const int block = p.group < kRowBlock ? kRowBlock : p.group;
   const int per = block / p.group;
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(M) + per - 1) / per));
