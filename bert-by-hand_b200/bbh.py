@@ -18,6 +18,7 @@ import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libbbh.so")
+OPS_PATH = os.path.join(HERE, "_bbh_ops.so")
 HIDDEN = 384
 
 BBH_OK = 0
@@ -541,171 +542,77 @@ def mean_pool_l2(hidden, cu_seqlens, tokmask=None, stream=None):
 # 16-bit tensors are float16 or bfloat16, all of one call the same; 2-D, unit stride along the
 # row, any row stride. The calls run on the tensors' device, on `stream` or that device's
 # current stream; outputs that are not given are allocated on that stream. Inference only:
-# no gradient is recorded.
-_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
-# the current stream's handle without building a torch.cuda.Stream (0.1 us instead of 3.3)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+# no gradient is recorded. The tensors are checked in the _bbh_ops module (csrc/torch_ops.cpp).
+_ops_module = None
 
 
-def _elsewhere(t, dev, stream):
-    """None, or the context that makes `stream` (None: the tensor's device's current one) and its
-    device current, when they are not."""
-    if dev < 0:
-        raise ValueError("expected a CUDA tensor")
-    if stream is not None:
-        if stream.device != t.device:
-            raise ValueError(f"the stream is on {stream.device}, the tensors are on {t.device}")
-        return torch.cuda.stream(stream)
-    return None if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+def _ops():
+    global _ops_module
+    if _ops_module is None:
+        import importlib.machinery
+        import importlib.util
+
+        lib()
+        if not os.path.exists(OPS_PATH):
+            raise RuntimeError(f"{OPS_PATH} is missing: build it with `python bert-by-hand_b200/build.py`")
+        loader = importlib.machinery.ExtensionFileLoader("_bbh_ops", OPS_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_bbh_ops", loader))
+        loader.exec_module(module)
+        module.set_error(BBHError)
+        _ops_module = module
+    return _ops_module
 
 
-def _rows(t, dev, dtype, shape, what):
-    """(data pointer, row stride) of a 2-D tensor, checked against dtype, shape and device."""
-    if t.dtype is not dtype:
-        raise TypeError(f"{what} must be {dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if t.get_device() != dev:
-        raise ValueError(f"{what} must be on cuda:{dev}")
-    ld, step = t.stride()
-    rows, cols = shape
-    if step != 1 and cols > 1:
-        raise ValueError(f"the rows of {what} must have unit stride")
-    # the stride of a single row says nothing
-    return t.data_ptr(), (ld if rows > 1 else (cols + 15) // 16 * 16)
-
-
-def _vector(t, dev, dtype, n, what):
-    """Data pointer of a contiguous vector of n elements, or None."""
-    if t is None:
-        return None
-    if t.dtype is not dtype:
-        raise TypeError(f"{what} must be {dtype}")
-    if t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous [{n}]")
-    if t.get_device() != dev:
-        raise ValueError(f"{what} must be on cuda:{dev}")
-    return t.data_ptr()
-
-
-def _new_i8(x, rows, cols):
-    """int8 [rows, cols] whose rows start at multiples of 16 bytes, as linear_i8 reads them, and their stride."""
-    ld = (cols + 15) // 16 * 16
-    q = x.new_empty((rows, ld), dtype=torch.int8)
-    return (q if ld == cols else q[:, :cols]), ld
-
-
-def _code(t):
-    if t.dim() != 2:
-        raise ValueError("expected a 2-D tensor")
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError("expected float16 or bfloat16")
-    return code
+def _on(t, stream):
+    """Context that makes `stream`, on t's device, the current one."""
+    if stream.device != t.device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors are on {t.device}")
+    return torch.cuda.stream(stream)
 
 
 def rmsnorm(x, weight=None, eps=1e-6, residual=None, out=None, sum_out=None, stream=None):
     """y = v / sqrt(mean(v^2) + eps) * weight with v = x + residual, in x's dtype; returns y, or
     (y, v) with a residual. out / sum_out receive them; each may be x or residual itself (the
     residual stream updated in place)."""
-    dev = x.get_device()
-    if (there := _elsewhere(x, dev, stream)) is not None:
-        with there:
+    if stream is not None:
+        with _on(x, stream):
             return rmsnorm(x, weight, eps, residual, out, sum_out)
-    code, dtype, shape = _code(x), x.dtype, x.shape
-    px, ldx = _rows(x, dev, dtype, shape, "x")
-    pr, ldr, ps, lds, v = None, 0, None, 0, None
-    if residual is not None:
-        pr, ldr = _rows(residual, dev, dtype, shape, "residual")
-        v = x.new_empty(shape) if sum_out is None else sum_out
-        ps, lds = (v.data_ptr(), shape[1]) if sum_out is None else _rows(v, dev, dtype, shape, "sum_out")
-    elif sum_out is not None:
-        raise ValueError("sum_out needs a residual")
-    y = x.new_empty(shape) if out is None else out
-    py, ldy = (y.data_ptr(), shape[1]) if out is None else _rows(y, dev, dtype, shape, "out")
-    _check(lib().bbh_rmsnorm(px, ldx, pr, ldr, _vector(weight, dev, dtype, shape[1], "weight"), py, ldy, ps, lds,
-                             shape[0], shape[1], eps, code, _raw_stream(dev)))
-    return y if residual is None else (y, v)
+    return (_ops_module or _ops()).rmsnorm(x, weight, eps, residual, out, sum_out)
 
 
 def rmsnorm_i8(x, weight=None, eps=1e-6, residual=None, sum_out=None, stream=None):
     """rmsnorm with the output in 8 bits: (q int8 [M, D], scale float32 [M]), or (q, scale, v) with a
     residual; y is q * scale. The rows of q start at multiples of 16 bytes (for linear_i8)."""
-    dev = x.get_device()
-    if (there := _elsewhere(x, dev, stream)) is not None:
-        with there:
+    if stream is not None:
+        with _on(x, stream):
             return rmsnorm_i8(x, weight, eps, residual, sum_out)
-    code, dtype, shape = _code(x), x.dtype, x.shape
-    M, D = shape
-    px, ldx = _rows(x, dev, dtype, shape, "x")
-    pr, ldr, ps, lds, v = None, 0, None, 0, None
-    if residual is not None:
-        pr, ldr = _rows(residual, dev, dtype, shape, "residual")
-        v = x.new_empty(shape) if sum_out is None else sum_out
-        ps, lds = (v.data_ptr(), D) if sum_out is None else _rows(v, dev, dtype, shape, "sum_out")
-    elif sum_out is not None:
-        raise ValueError("sum_out needs a residual")
-    q, ldq = _new_i8(x, M, D)
-    scale = x.new_empty((M,), dtype=torch.float32)
-    _check(lib().bbh_rmsnorm_i8(px, ldx, pr, ldr, _vector(weight, dev, dtype, D, "weight"), q.data_ptr(), ldq,
-                                scale.data_ptr(), ps, lds, M, D, eps, code, _raw_stream(dev)))
-    return (q, scale) if residual is None else (q, scale, v)
+    return (_ops_module or _ops()).rmsnorm_i8(x, weight, eps, residual, sum_out)
 
 
 def quantize_i8(x, stream=None):
     """Rows of x [M, D] in 8 bits: (q int8 [M, D], scale float32 [M]), x ~ q * scale. Activations (a scale
     per token) or nn.Linear weights (a scale per output channel)."""
-    dev = x.get_device()
-    if (there := _elsewhere(x, dev, stream)) is not None:
-        with there:
+    if stream is not None:
+        with _on(x, stream):
             return quantize_i8(x)
-    code = _code(x)
-    M, D = x.shape
-    px, ldx = _rows(x, dev, x.dtype, x.shape, "x")
-    q, ldq = _new_i8(x, M, D)
-    scale = x.new_empty((M,), dtype=torch.float32)
-    _check(lib().bbh_quantize_i8(px, ldx, q.data_ptr(), ldq, scale.data_ptr(), M, D, code, _raw_stream(dev)))
-    return q, scale
+    return (_ops_module or _ops()).quantize_i8(x)
 
 
 def dequantize_i8(q, scale, dtype=torch.float16, out=None, stream=None):
     """q * scale[:, None] in dtype (out's, if given)."""
-    dev = q.get_device()
-    if (there := _elsewhere(q, dev, stream)) is not None:
-        with there:
+    if stream is not None:
+        with _on(q, stream):
             return dequantize_i8(q, scale, dtype, out)
-    if q.dim() != 2:
-        raise ValueError("expected a 2-D tensor")
-    shape = q.shape
-    pq, ldq = _rows(q, dev, torch.int8, shape, "q")
-    y = q.new_empty(shape, dtype=dtype) if out is None else out
-    code = _code(y)
-    py, ldy = (y.data_ptr(), shape[1]) if out is None else _rows(y, dev, y.dtype, shape, "out")
-    _check(lib().bbh_dequantize_i8(pq, ldq, _vector(scale, dev, torch.float32, shape[0], "scale"), py, ldy, shape[0],
-                                   shape[1], code, _raw_stream(dev)))
-    return y
+    return (_ops_module or _ops()).dequantize_i8(q, scale, dtype, out)
 
 
 def linear_i8(A, a_scale, W, w_scale, bias=None, gelu=False, dtype=torch.float16, out=None, stream=None):
     """(A [M, K] @ W [N, K]^T) * a_scale[:, None] * w_scale (+ bias) (+ erf-GELU) in dtype (out's, if given); A, W
     int8 with rows at multiples of 16 bytes, as quantize_i8 and rmsnorm_i8 return them."""
-    dev = A.get_device()
-    if (there := _elsewhere(A, dev, stream)) is not None:
-        with there:
+    if stream is not None:
+        with _on(A, stream):
             return linear_i8(A, a_scale, W, w_scale, bias, gelu, dtype, out)
-    if A.dim() != 2 or W.dim() != 2:
-        raise ValueError("A and W must be 2-D")
-    M, K = A.shape
-    N = W.shape[0]
-    pa, lda = _rows(A, dev, torch.int8, A.shape, "A")
-    pw, ldw = _rows(W, dev, torch.int8, (N, K), "W")
-    C = A.new_empty((M, N), dtype=dtype) if out is None else out
-    code = _code(C)
-    pc, ldc = (C.data_ptr(), N) if out is None else _rows(C, dev, C.dtype, (M, N), "out")
-    _check(lib().bbh_linear_i8(pa, lda, _vector(a_scale, dev, torch.float32, M, "a_scale"), pw, ldw,
-                               _vector(w_scale, dev, torch.float32, N, "w_scale"), _vector(bias, dev, C.dtype, N, "bias"),
-                               pc, ldc, M, N, K, 1 if gelu else 0, code, _raw_stream(dev)))
-    return C
+    return (_ops_module or _ops()).linear_i8(A, a_scale, W, w_scale, bias, gelu, dtype, out)
 
 
 def linear_i8_device_error(reset: bool = True) -> int:

@@ -2,7 +2,8 @@
 
 Each .cu in csrc/ is compiled to an object (in parallel), then linked into a shared
 library with the CUDA runtime linked statically, so the library loads on a machine
-without a GPU driver (its calls then fail with BBH_ERR_CUDA / BBH_ERR_UNSUPPORTED).
+without a GPU driver (its calls then fail with BBH_ERR_CUDA / BBH_ERR_UNSUPPORTED). The
+_bbh_ops Python module (csrc/torch_ops.cpp) is compiled with the host compiler against torch.
 """
 from __future__ import annotations
 
@@ -61,6 +62,33 @@ def build(verbose_ptxas: bool = False) -> str:
     return LIB
 
 
+OPS_SRC = os.path.join(CSRC, "torch_ops.cpp")
+OPS = os.path.join(HERE, "_bbh_ops.so")
+CXX = os.environ.get("CXX", "g++")
+
+
+def build_ops() -> str:
+    """The _bbh_ops Python module: torch tensors in front of libbbh.so's 8-bit operators (rpath = its folder)."""
+    lib = build()
+    deps = [OPS_SRC, os.path.join(HERE, "..", "include", "bbh.h")]
+    if _needs(OPS, deps):
+        import sysconfig
+
+        import torch
+
+        root = os.path.dirname(torch.__file__)
+        inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+        cmd = [CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *["-isystem" + i for i in inc],
+               OPS_SRC, "-o", OPS, "-L" + os.path.dirname(lib), "-lbbh", "-L" + os.path.join(root, "lib"), "-lc10",
+               "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"_bbh_ops build failed:\n{r.stdout}\n{r.stderr}")
+    return OPS
+
+
 EXAMPLE_SRC = os.path.join(HERE, "examples", "bert_embed_main.cpp")
 EXAMPLE_BIN = os.path.join(OBJ, "bert_embed_main")
 
@@ -80,4 +108,5 @@ def build_example() -> str:
 
 if __name__ == "__main__":
     print(build(verbose_ptxas="-v" in sys.argv))
+    print(build_ops())
     print(build_example())
