@@ -213,7 +213,7 @@ struct I8PairCfg {
   static_assert((2 * STAGES + 2 * NACC) * 8 + 8 <= 512, "barriers");
 };
 
-// TMA_C: C is written with TMA stores (16-byte aligned rows); otherwise row by row from the
+// TMA_C: C is written with TMA stores (16-byte aligned rows of whole 16 bytes); otherwise row by row from the
 // staging buffer with 2-byte stores, which any N and alignment allows.
 template <int BN, int COLS, bool BF16, bool GELU, bool TMA_C>
 __global__ void __launch_bounds__(I8PairCfg<BN, COLS>::THREADS, 1)
@@ -926,7 +926,8 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
 
   I8Params p{a_scale, w_scale, bias, C, ldc, M, N, K};
   const bool bf16 = dtype == BBH_BF16, g = gelu != 0;
-  const bool tma_c = !(bits(C) & 15) && ldc % 8 == 0;
+  // N % 8: a TMA store ends at a 16-byte boundary, not inside one (it overwrote up to 7 elements of padding)
+  const bool tma_c = !(bits(C) & 15) && ldc % 8 == 0 && N % 8 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   I8Maps maps;
   cudaError_t e;

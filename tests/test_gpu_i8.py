@@ -397,7 +397,8 @@ def test_linear_i8_bits_do_not_depend_on_the_batch(N, K, dtype):
 
 
 @pytest.mark.parametrize("M,N,ldc,offset", [(5, 100, 128, 0), (5, 100, 101, 1), (300, 384, 400, 8), (3000, 1536, 1544, 0),
-                                            (3000, 1500, 1537, 3), (2900, 1152, 1156, 0)])
+                                            (3000, 1500, 1537, 3), (2900, 1152, 1156, 0), (3000, 1529, 1536, 0),
+                                            (3786, 2095, 2096, 8), (2900, 1340, 1344, 0)])
 def test_linear_i8_output_strides(M, N, ldc, offset):
     """C of any stride and alignment; what lies around it stays."""
     import bbh
