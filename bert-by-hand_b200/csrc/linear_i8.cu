@@ -3,12 +3,13 @@
 // The sum is exact (tcgen05.mma kind::i8, int32 accumulators in TMEM; |sum| <= 128^2 K < 2^31
 // for K <= 131071), so the result does not depend on tile shape, split or order.
 //
-// Two kernels, both fed by 128-byte-swizzled TMA tiles of 128 int8 along K:
+// Three kernels:
 //  * linear_i8_pair_kernel -- many rows: persistent SM pairs (cta_group::2) on 256 x BN tiles,
 //    two TMEM accumulators so that the epilogue of a tile runs under the MMAs of the next;
 //  * linear_i8_small_kernel -- few rows: the weights are the MMA's 128-row operand and BN tokens
 //    its columns, K split over the CTAs of a cluster, partial sums added in shared memory
-//    (int32: exact in any order).
+//    (int32: exact in any order); both fed by 128-byte-swizzled TMA tiles of 128 int8 along K;
+//  * linear_i8_few_kernel -- one to 16 tokens: the weights straight from memory into registers.
 // Every wait is bounded (mbar_wait); one that runs out sets the device error word and the
 // kernel returns.
 #include "common.cuh"
@@ -762,6 +763,108 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
   }
 }
 
+// ======================================================================== one to 16 tokens
+
+// Single tokens and decoding batches: the weights' bytes are the work, and a launch's fixed costs (TMEM,
+// barriers, a cluster) are as long as their transfer. So no staging: a CTA has 16 output channels, its
+// eight warps every eighth 64 bytes of K, loaded straight into the fragments of mma.sync m16n8k32 (the
+// order of k is free as long as both operands have the same, so a lane's 16 consecutive bytes are four
+// of its fragments' words), and the partial sums meet in shared memory. 1 x 4096 x 4096: 3.3 us = 5.1 TB/s
+// of weights (they fit in L2 when repeated), 1 x 8192 x 8192 9.4 us = 7.1 TB/s.
+constexpr int kFewWarps = 8;
+
+__device__ __forceinline__ void mma_i8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bytes of an int8 row from k on, zeros behind its end (and nothing read there).
+__device__ __forceinline__ uint4 load_k16(const int8_t* row, int k, int K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  const int r = k < K ? K - k : 0;  // 0 .. 15 bytes: an 8-, a 4-, a 2- and a 1-byte load
+  const int8_t* at = row + k;
+  uint64_t lo = 0, rest = 0;
+  if (r & 8) lo = *reinterpret_cast<const uint64_t*>(at);
+  at += r & 8;
+  if (r & 4) rest = *reinterpret_cast<const uint32_t*>(at);
+  at += r & 4;
+  if (r & 2) rest |= static_cast<uint64_t>(*reinterpret_cast<const uint16_t*>(at)) << (8 * (r & 4));
+  at += r & 2;
+  if (r & 1) rest |= static_cast<uint64_t>(static_cast<uint8_t>(*at)) << (8 * (r & 6));
+  const uint64_t hi = r & 8 ? rest : 0;
+  lo = r & 8 ? lo : rest;
+  return make_uint4(static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
+                    static_cast<uint32_t>(hi >> 32));
+}
+
+// MT: token tiles of 8. U: 64-byte steps in flight per warp.
+template <int MT, int U, bool BF16, bool GELU>
+__global__ void __launch_bounds__(32 * kFewWarps)
+    linear_i8_few_kernel(const int8_t* __restrict__ A, const int64_t lda, const int8_t* __restrict__ W,
+                         const int64_t ldw, const I8Params p) {
+  __shared__ int part[kFewWarps][MT * 128];
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, q = lane & 3;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  // rows behind the last channel or token repeat the last one; their sums are not used
+  const int8_t* w0 = W + min(n0 + g, static_cast<int64_t>(p.N) - 1) * ldw;
+  const int8_t* w1 = W + min(n0 + g + 8, static_cast<int64_t>(p.N) - 1) * ldw;
+  const int8_t* x[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) x[t] = A + static_cast<int64_t>(min(8 * t + g, p.M - 1)) * lda;
+  int acc[MT][4] = {};
+  pdl_wait();
+  for (int k0 = 64 * warp; k0 < p.K; k0 += 64 * kFewWarps * U) {
+    uint4 a[U], b[U], v[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + 64 * kFewWarps * u + 16 * q;
+      a[u] = load_k16(w0, k, p.K);
+      b[u] = load_k16(w1, k, p.K);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) v[u][t] = load_k16(x[t], k, p.K);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        mma_i8(acc[t], a[u].x, b[u].x, a[u].y, b[u].y, v[u][t].x, v[u][t].y);
+        mma_i8(acc[t], a[u].z, b[u].z, a[u].w, b[u].w, v[u][t].z, v[u][t].w);
+      }
+  }
+  // acc[t]: channels g (0, 1) and g + 8 (2, 3), tokens 8 t + 2 q and the next; part[warp][token][channel]
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[warp][(8 * t + 2 * q + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[t][i];
+  __syncthreads();
+  // one thread a token and two neighbouring channels
+  const int tok = threadIdx.x >> 3, c = 2 * (threadIdx.x & 7);
+  if (tok >= p.M || tok >= 8 * MT) return;
+  int s0 = 0, s1 = 0;
+#pragma unroll
+  for (int w = 0; w < kFewWarps; ++w) {
+    const int2 u = *reinterpret_cast<const int2*>(&part[w][tok * 16 + c]);
+    s0 += u.x;
+    s1 += u.y;
+  }
+  const int64_t n = n0 + c;
+  const bool one = n < p.N, two = n + 1 < p.N;
+  const float sa = __ldg(p.a_scale + tok);
+  const float b0 = p.bias && one ? bias_f32<BF16>(p.bias + n) : 0.f, b1 = p.bias && two ? bias_f32<BF16>(p.bias + n + 1) : 0.f;
+  unsigned long long y[1] = {dequant2(s0, s1, f2(sa, sa), f2(one ? __ldg(p.w_scale + n) : 0.f, two ? __ldg(p.w_scale + n + 1) : 0.f),
+                                      f2(b0, b1))};
+  uint32_t o[1];
+  finish2<BF16, GELU>(y, o);
+  uint16_t* out = p.C + tok * p.ldc + n;
+  if (one) out[0] = static_cast<uint16_t>(o[0]);
+  if (two) out[1] = static_cast<uint16_t>(o[0] >> 16);
+}
+
 // ======================================================================== host side
 namespace {
 
@@ -860,6 +963,34 @@ cudaError_t launch_small_bn(const I8Maps& m, const I8Params& p, bool bf16, bool 
               : launch_small_i8<BN, false, false>(m, p, log_splits, dev, s);
 }
 
+template <int MT, int U>
+cudaError_t launch_few(const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, const I8Params& p, bool bf16,
+                       bool gelu, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((int64_t(p.N) + 15) / 16));
+  auto go = [&](auto kern) { return launch_ex(kern, grid, dim3(32 * kFewWarps), 0, s, true, 1, A, lda, W, ldw, p); };
+  if (bf16) return gelu ? go(linear_i8_few_kernel<MT, U, true, true>) : go(linear_i8_few_kernel<MT, U, true, false>);
+  return gelu ? go(linear_i8_few_kernel<MT, U, false, true>) : go(linear_i8_few_kernel<MT, U, false, false>);
+}
+
+// Steps in flight: as many as a warp has (512 bytes of K each), where the CTAs are too few to keep memory
+// busy otherwise. 1 x 4096 x 4096: 8 steps 3.3 us, 4 steps 4.0, 2 steps 4.7; 1 x 384 x 384: 2.5, 1.9, 1.5;
+// 1 x 16384 x 4096 (1,024 CTAs): 10.3, 9.8, 9.2.
+cudaError_t launch_few_any(const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, const I8Params& p, bool bf16,
+                           bool gelu, int sms, cudaStream_t s) {
+  if (p.M > 8) return launch_few<2, 2>(A, lda, W, ldw, p, bf16, gelu, s);
+  if (p.K <= 1024 || p.N > 32 * sms) return launch_few<1, 2>(A, lda, W, ldw, p, bf16, gelu, s);
+  return p.K <= 2048 ? launch_few<1, 4>(A, lda, W, ldw, p, bf16, gelu, s)
+                     : launch_few<1, 8>(A, lda, W, ldw, p, bf16, gelu, s);
+}
+
+// Whether that kernel takes less time than the tcgen05 one (us, few rows / tcgen05): 1 x 4096 x 4096 3.3 / 4.6;
+// 4 x 16384 x 4096 9.8 / 9.8; 8 x 4096 x 4096 3.6 / 4.6; 8 x 16384 x 4096 10.5 / 9.8; 16 x 1536 x 384 2.0 / 2.6;
+// 16 x 4096 x 1024 2.9 / 3.3; 16 x 1024 x 8192 6.6 / 4.8; 16 x 4096 x 4096 5.1 / 4.8.
+bool few_is_faster(int M, int N, int K) {
+  const int64_t weights = int64_t(N) * K;
+  return M <= 4 || (M <= 8 && weights <= (int64_t(32) << 20)) || (M <= 16 && K <= 2048 && weights <= (int64_t(4) << 20));
+}
+
 struct I8Plan {
   bool pair;
   int bn;          // column tile of the pair kernel, token tile of the other
@@ -932,7 +1063,9 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
   I8Maps maps;
   cudaError_t e;
   const I8Plan plan = choose_plan(M, N, K, sms);
-  if (!plan.pair) {
+  if (few_is_faster(M, N, K)) {
+    e = launch_few_any(A, lda, W, ldw, p, bf16, g, sms, s);
+  } else if (!plan.pair) {
     rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, plan.bn, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return internal_fail(rc, "bbh_linear_i8: tensor map encoding failed");

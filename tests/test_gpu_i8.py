@@ -313,7 +313,8 @@ LINEAR = [(1, 1, 1), (1, 16, 16), (1, 384, 384), (2, 130, 100), (5, 1000, 31), (
           (32, 4096, 1024), (33, 256, 4096), (64, 1152, 384), (65, 1536, 384), (127, 999, 1537), (128, 384, 1536),
           (129, 8, 5000), (200, 257, 640), (1000, 1152, 384), (1024, 1024, 1024), (777, 1001, 333), (3000, 384, 1536),
           (2500, 1536, 384), (2049, 2047, 127), (4100, 1344, 200), (3001, 1152, 17), (70000, 24, 64), (24, 70000, 64),
-          (9, 64, 131071)]
+          (9, 64, 131071), (1, 4096, 4096), (4, 5000, 2048), (8, 300, 8000), (8, 33, 65), (7, 15, 515), (9, 17, 1000),
+          (16, 1024, 1040), (1, 70001, 48), (3, 2000, 4104)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -391,7 +392,7 @@ def test_linear_i8_bits_do_not_depend_on_the_batch(N, K, dtype):
     a, sa, w, sw, b = make_linear(5000, N, K, dtype, True)
     for gelu in (False, True):
         full = bbh.linear_i8(a, sa, w, sw, b, gelu=gelu, dtype=dtype)
-        for m in (1, 15, 32, 50, 128, 300, 1100):
+        for m in (1, 8, 11, 15, 32, 50, 128, 300, 1100):
             part = bbh.linear_i8(a[:m], sa[:m], w, sw, b, gelu=gelu, dtype=dtype)
             assert torch.equal(part, full[:m]), (m, gelu)
 
