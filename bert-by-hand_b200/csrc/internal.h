@@ -54,17 +54,24 @@ cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t sm
 int internal_fail(int code, const std::string& msg);
 // The calling thread's current device, which has to be an sm_100, and its SM count.
 int unit_device(int* device, int* num_sms);
-// Rows [rows, cols] of `bytes`-wide elements, `ld` elements apart: the first byte, the one
-// behind the last, and the stride; for refusing outputs that overlap inputs. rows >= 1.
+// Rows [rows, cols] of `bytes`-wide elements, `ld` >= cols elements apart: the first byte, the one
+// behind the last, and a row's distance and width in bytes; for refusing outputs that overlap
+// inputs. rows >= 1.
 struct Span {
-  uintptr_t lo, hi;
-  int64_t ld;
+  uintptr_t lo, hi, step, width;
 };
 inline Span span(const void* p, int64_t ld, int rows, int cols, int bytes) {
-  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-  return {lo, lo + (uintptr_t(rows - 1) * uintptr_t(ld) + uintptr_t(cols)) * uintptr_t(bytes), ld};
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p), step = uintptr_t(ld) * bytes, width = uintptr_t(cols) * bytes;
+  return {lo, lo + uintptr_t(rows - 1) * step + width, step, width};
 }
-inline bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+// Rows of one distance may lie between one another (columns of the same matrix); of different
+// distances, they overlap if their ranges do.
+inline bool overlap(const Span& a, const Span& b) {
+  if (a.lo >= b.hi || b.lo >= a.hi) return false;
+  if (a.step != b.step) return true;
+  const uintptr_t d = b.lo >= a.lo ? (b.lo - a.lo) % a.step : (a.step - (a.lo - b.lo) % a.step) % a.step;
+  return d < a.width || d + b.width > a.step;
+}
 // Device and capacity of a workspace.
 void ws_limits(const bbh_ws* ws, int* device, int* max_tokens, int* max_batch, int* max_len);
 // The workspace's slot for the corpus driver's staging state; free_fn releases it when

@@ -769,8 +769,8 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
 // barriers, a cluster) are as long as their transfer. So no staging: a CTA has 16 output channels, its
 // eight warps every eighth 64 bytes of K, loaded straight into the fragments of mma.sync m16n8k32 (the
 // order of k is free as long as both operands have the same, so a lane's 16 consecutive bytes are four
-// of its fragments' words), and the partial sums meet in shared memory. 1 x 4096 x 4096: 3.3 us = 5.1 TB/s
-// of weights (they fit in L2 when repeated), 1 x 8192 x 8192 9.4 us = 7.1 TB/s.
+// of its fragments' words), and the partial sums meet in shared memory. 1 x 4096 x 4096: 3.2 us = 5.2 TB/s
+// of weights (they fit in L2 when repeated), 1 x 8192 x 8192 8.2 us = 8.2 TB/s.
 constexpr int kFewWarps = 8;
 
 __device__ __forceinline__ void mma_i8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,

@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
       ties = (((__float_as_uint(top) >> 13) & 0x3ffu) | 0x400u) % 127u == 0;
       if (ties) rest = fmaf(-inv, top, 127.f) / top;
     }
-    if (live && t == 0) p.scale[r] = finite ? (zero ? 0.f : top / 127.f) * rstd : __int_as_float(0x7fc00000);
+    if (live && t == 0) p.scale[r] = !finite ? __int_as_float(0x7fc00000) : zero ? 0.f : top / 127.f * rstd;
     int8_t* q = p.q + r * p.ldq;
     if constexpr (CUT == kShifted) {
       // The bytes of a chunk are not where an aligned store of q wants them: through shared memory, element e
@@ -545,7 +545,7 @@ bool off(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p)
 // is written, by one thread); any other overlap is refused.
 bool clash(const Span& out, const void* out_p, const Span& in, const void* in_p, bool same_ok) {
   if (!in_p || !out_p || !overlap(out, in)) return false;
-  return !(same_ok && out.lo == in.lo && out.ld == in.ld);
+  return !(same_ok && out.lo == in.lo && out.step == in.step);
 }
 
 int check_rows(const char* who, int rows, int D, int dtype) {

@@ -203,7 +203,8 @@ BBH_API int bbh_mean_pool_l2(const uint16_t* hidden, const int32_t* cu_seqlens, 
 #define BBH_LINEAR_I8_MAX_K 131071
 /* v = x + residual (fp32, not rounded; residual may be NULL); y = v / sqrt(mean(v^2) + eps) *
  * weight (NULL: ones). sum (NULL, or with a residual) receives v rounded to dtype. y and sum
- * may each be x or residual itself (same pointer, same stride). D in [1, 32768]. */
+ * may each be x or residual itself (same pointer, same stride). D in [1, 32768]. The squares are
+ * fp32 too: a row whose sum of squares is above 3.4e38 (bf16 reaches it) gives y = 0. */
 BBH_API int bbh_rmsnorm(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr, const uint16_t* weight,
                         uint16_t* y, int64_t ldy, uint16_t* sum, int64_t lds, int M, int D, float eps, int dtype,
                         void* stream);
@@ -222,10 +223,9 @@ BBH_API int bbh_quantize_i8(const uint16_t* x, int64_t ldx, int8_t* q, int64_t l
 BBH_API int bbh_dequantize_i8(const int8_t* q, int64_t ldq, const float* scale, uint16_t* y, int64_t ldy, int M, int D,
                               int dtype, void* stream);
 /* C[M, N] = (A W^T) * a_scale[m] * w_scale[n] (+ bias[n]) (+ erf-GELU, within 1e-6 max(|x|, 1) of
- * the exact form before the rounding), A [M, K] and W [N, K] (nn.Linear layout) int8, exact int32
- * sums. A and W 16-byte aligned with row
- * strides of whole 16 bytes (K itself may be any value in [1, 131071]); C and bias (dtype, bias
- * may be NULL) of any alignment and N. */
+ * the exact form before the rounding; NaN for an infinite x), A [M, K] and W [N, K] (nn.Linear layout)
+ * int8, exact int32 sums. A and W 16-byte aligned with row strides of whole 16 bytes (K itself may be
+ * any value in [1, 131071]); C and bias (dtype, bias may be NULL) of any alignment and N. */
 BBH_API int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw,
                           const float* w_scale, const uint16_t* bias, uint16_t* C, int64_t ldc, int M, int N, int K,
                           int gelu, int dtype, void* stream);

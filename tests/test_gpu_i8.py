@@ -261,6 +261,36 @@ def test_special_rows(D, dtype):
     assert bool(torch.isnan(c[3:6]).all()) and bool(torch.isfinite(c[[0, 1, 2, 6, 7]]).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [16, 77, 4096])
+def test_zero_rows_with_eps_zero(D, dtype):
+    """1 / sqrt(0) is infinite; a zero row still gets scale 0 and zeros."""
+    import bbh
+
+    x = rows16(5, D, dtype, gen("zeros", D))
+    x[[1, 4]] = 0
+    q, s, v = bbh.rmsnorm_i8(x, eps=0.0, residual=torch.zeros_like(x))
+    assert s[[1, 4]].tolist() == [0, 0] and bool((q[[1, 4]] == 0).all()) and torch.equal(v, x)
+    assert bool((s[[0, 2, 3]] > 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,D", [(1, 64), (7, 384), (300, 1000)])
+def test_columns_of_one_matrix(M, D, dtype):
+    """Operands that are columns of the same matrix: the same bits as separate ones, nothing else written."""
+    import bbh
+
+    g = gen("columns", M, D)
+    x, r = rows16(M, D, dtype, g), rows16(M, D, dtype, g)
+    y, v = bbh.rmsnorm(x, residual=r)
+    wide = torch.full((M, 4 * D + 8), 7, dtype=dtype, device=DEV)
+    part = [wide[:, i * D:(i + 1) * D] for i in range(4)]
+    part[0].copy_(x)
+    part[2].copy_(r)
+    bbh.rmsnorm(part[0], residual=part[2], out=part[1], sum_out=part[3])
+    assert all(torch.equal(a, b) for a, b in zip(part, (x, y, r, v))) and bool((wide[:, 4 * D:] == 7).all())
+
+
 def test_rows_past_32_bit_offsets():
     """2.25 G elements: the last rows are those of a small call."""
     import bbh
@@ -540,6 +570,43 @@ def test_captured_and_replayed(M):
         for graph, x, r, nw, up, down, y, v in graphs:
             y0, v0 = ffn(bbh, x, r, nw, up, down)
             assert torch.equal(y, y0) and torch.equal(v, v0)
+
+
+_FIRST_CALLS = """
+import sys
+sys.path[:0] = [{here!r}]
+import torch, bbh
+g = torch.Generator().manual_seed(1)
+x = torch.randn(40, 256, generator=g).half().cuda()
+w = torch.randn(512, 256, generator=g).half().cuda()
+many = x.repeat(60, 1)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    wq, ws = bbh.quantize_i8(w)
+    outs = [bbh.linear_i8(*bbh.rmsnorm_i8(t), wq, ws, gelu=True) for t in (x[:1], x, many)]
+    outs.append(bbh.dequantize_i8(wq, ws))
+graph.replay()
+wq, ws = bbh.quantize_i8(w)
+eager = [bbh.linear_i8(*bbh.rmsnorm_i8(t), wq, ws, gelu=True) for t in (x[:1], x, many)]
+eager.append(bbh.dequantize_i8(wq, ws))
+assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+assert bbh.linear_i8_device_error() == 0
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_captured():
+    """What a kernel's first launch sets up once may happen while a stream is captured."""
+    import os
+    import subprocess
+    import sys
+
+    import bbh
+
+    code = _FIRST_CALLS.format(here=os.path.dirname(os.path.abspath(bbh.__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stdout + r.stderr
 
 
 def test_two_streams_at_once():

@@ -111,3 +111,25 @@ def test_entry_points_return_codes_not_exceptions():
     assert L.bbh_rmsnorm(None, 0, None, 0, None, None, 0, None, 0, 1, 1, 0.0, 0, None) == ARG
     assert L.bbh_linear_i8(None, 0, None, None, 0, None, None, None, 0, 1, 1, 1, 0, 0, None) == ARG
     assert isinstance(ctypes.string_at(L.bbh_last_error()), bytes)
+
+
+COLUMNS = [("rmsnorm", dict(ldx=192, ldr=192, r=X + 128, ldy=192, y=X + 256)),
+           ("rmsnorm", dict(ldx=192, x=X + 128, y=X, ldy=192)), ("rmsnorm", dict(ldx=192, s=X + 128, lds=192)),
+           ("quantize", dict(ldx=96, q=X + 128, ldq=192)),
+           ("dequantize", dict(ldq=256, y=Q + 64, ldy=128)),
+           ("linear", dict(lda=128, C=X + 64, ldc=64))]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are not real")
+@pytest.mark.parametrize("name,args", COLUMNS)
+def test_columns_of_one_matrix_do_not_overlap(name, args):
+    assert CALLS[name](**args) in (CUDA, UNSUPPORTED)
+
+
+@pytest.mark.parametrize("name,args", [
+    ("rmsnorm", dict(ldx=192, y=X + 126, ldy=192)), ("rmsnorm", dict(ldx=192, y=X + 258, ldy=192)),
+    ("rmsnorm", dict(ldx=192, x=X + 128, y=X + 2, ldy=192)), ("rmsnorm", dict(ldx=192, y=X + 128, ldy=193)),
+    ("quantize", dict(ldx=96, q=X + 127, ldq=192)), ("quantize", dict(ldx=96, q=X + 129, ldq=192)),
+    ("linear", dict(lda=128, C=X + 62, ldc=64)), ("linear", dict(lda=128, C=X + 66, ldc=64))])
+def test_columns_that_meet_are_refused(name, args):
+    assert CALLS[name](**args) == ARG and "overlap" in message()
