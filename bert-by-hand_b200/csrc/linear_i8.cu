@@ -76,7 +76,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // One lane of a converged warp. The loops that issue copies and MMAs run under it and not under
 // `lane == 0`: it tells the compiler that a single lane runs them, and their descriptors and addresses
 // stay in uniform registers. An MMA then takes its thread 30 cycles instead of 60 and a k-block of
-// the few-rows kernel 245 to 316 instead of 460 (which was its time for any number of tokens).
+// the few-rows kernel 245 to 316 instead of 460 (which it took for any number of tokens).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -723,8 +723,12 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
           const int t = c + 4 * g;
           if (t < tokens) {
             const int piece = (t & ((1 << log_per) - 1)) >> 2;
-            const uint32_t at = smem_u32(red) + ((rank * pieces + piece) * 128 + ch) * 16;
-            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_shared(at, t >> log_per)),
+            int4* at = reinterpret_cast<int4*>(red) + (rank * pieces + piece) * 128 + ch;
+            if (t >> log_per == rank) {
+              *at = a[g];
+              continue;
+            }
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_shared(smem_u32(at), t >> log_per)),
                          "r"(a[g].x), "r"(a[g].y), "r"(a[g].z), "r"(a[g].w)
                          : "memory");
           }
@@ -899,17 +903,17 @@ cudaError_t opt_in(K kern, int smem, bool (&done)[64], int dev) {
   return e;
 }
 
-// Pairs of SMs that can run a kernel at once, asked once per device and kernel.
+// Clusters of `size` CTAs that can run at once, asked once per device and kernel.
 template <typename K>
-int max_pairs(K kern, int threads, int smem, int sms, int (&cache)[64], int dev) {
+int max_clusters(K kern, int size, int threads, int smem, int sms, int (&cache)[64], int dev) {
   if (cache[dev]) return cache[dev];
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = size;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(sms & ~1);
+  cfg.gridDim = dim3(sms / size * size);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.attrs = attr;
@@ -917,7 +921,7 @@ int max_pairs(K kern, int threads, int smem, int sms, int (&cache)[64], int dev)
   int n = 0;
   if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
     (void)cudaGetLastError();
-    n = sms / 2;
+    n = sms / size;
   }
   return cache[dev] = n;
 }
@@ -935,7 +939,7 @@ cudaError_t launch_pair_i8(const I8Maps& m, const I8Params& p, int dev, int sms,
   if (e != cudaSuccess) return e;
   static int pairs_of[64] = {};
   const int64_t tiles = (int64_t(p.M) + 255) / 256 * ((p.N - 1) / BN + 1);
-  const int most = max_pairs(kern, Cfg::THREADS, Cfg::SMEM, sms, pairs_of, dev);
+  const int most = max_clusters(kern, 2, Cfg::THREADS, Cfg::SMEM, sms, pairs_of, dev);
   const int pairs = static_cast<int>(tiles < most ? tiles : most);
   return launch_ex(kern, dim3(2 * pairs), dim3(Cfg::THREADS), Cfg::SMEM, s, true, 2, m.A, m.W, m.C, p);
 }
@@ -1005,12 +1009,13 @@ cudaError_t launch_few_any(const int8_t* A, int64_t lda, const int8_t* W, int64_
                      : launch_few<1, 8>(A, lda, W, ldw, p, bf16, gelu, s);
 }
 
-// Whether that kernel takes less time than the tcgen05 one (us, few rows / tcgen05): 1 x 4096 x 4096 3.3 / 4.6;
-// 4 x 16384 x 4096 9.8 / 9.8; 8 x 4096 x 4096 3.6 / 4.6; 8 x 16384 x 4096 10.5 / 9.8; 16 x 1536 x 384 2.0 / 2.6;
-// 16 x 4096 x 1024 2.9 / 3.3; 16 x 1024 x 8192 6.6 / 4.8; 16 x 4096 x 4096 5.1 / 4.8.
-bool few_is_faster(int M, int N, int K) {
+// Whether that kernel takes less time than the tcgen05 one (us, few rows / tcgen05): 1 x 4096 x 4096 3.3 / 4.1;
+// 1 x 2048 x 8192 4.7 / 4.4; 4 x 16384 x 4096 8.8 / 8.7; 8 x 4096 x 4096 3.6 / 4.0; 8 x 16384 x 4096 9.5 / 7.3;
+// 16 x 1536 x 384 2.3 / 2.3; 16 x 1024 x 1024 2.1 / 2.9; 16 x 1024 x 4096 3.8 / 3.3; 16 x 4096 x 4096 5.6 / 4.0.
+bool few_is_faster(int M, int N, int K, int sms) {
   const int64_t weights = int64_t(N) * K;
-  return M <= 4 || (M <= 8 && weights <= (int64_t(32) << 20)) || (M <= 16 && K <= 2048 && weights <= (int64_t(4) << 20));
+  if (M <= 8) return (M <= 4 || weights <= (int64_t(16) << 20)) && (K <= 4096 || N > 16 * sms);
+  return M <= 16 && K <= 2048 && weights <= (int64_t(4) << 20);
 }
 
 struct I8Plan {
@@ -1019,25 +1024,40 @@ struct I8Plan {
   int log_splits;  // K split over 2^log_splits CTAs
 };
 
-// The kernel and tile that take the least time by this model of a launch, in us, fitted to times of
-// back-to-back launches on a B200 (sizes from 16 to 2048 rows, 384 to 8192 columns, K to 8192; it is
-// within about 10 % of them and picks the fastest or one within 5 % of it):
-//   few rows: 1.65 + 0.0113 bn + 0.235 k-blocks per CTA, and 0.7 + 0.008 bn log2(splits) for a split K (the
-//     cluster's barriers and the exchange of partial sums), every CTA on an SM of its own;
-//   pairs: 3.9 + 0.28 k-blocks per round of tiles.
-// E.g. 64 x 4096 x 4096: bn 64 in 4 parts 6.1 us, bn 32 in 2 parts 6.8, bn 64 whole 9.9, pairs 12.7;
-// 1000 x 1000 x 1000: bn 64 whole 5.0 us, bn 128 in 2 parts 6.3, pairs 7.7.
-I8Plan choose_plan(int M, int N, int K, int sms) {
+// CTAs of the few-rows kernel that run at once in clusters of 2^log_splits, in clusters (all token tiles
+// have an SM to themselves, so one of them answers for all): 148, 74, 33 and 15 on a B200, whose parts
+// do not all hold a whole number of large clusters.
+int cluster_room(int log_splits, int sms, int dev) {
+  using Cfg = I8SmallCfg<64>;
+  static bool done[64] = {};
+  static int room[4][64] = {};
+  if (log_splits == 0) return sms;
+  auto kern = linear_i8_small_kernel<64, false, false>;
+  if (opt_in(kern, Cfg::SMEM, done, dev) != cudaSuccess) return sms >> log_splits;
+  return max_clusters(kern, 1 << log_splits, Cfg::THREADS, Cfg::SMEM, sms, room[log_splits], dev);
+}
+
+// The kernel and tile that take the least time by this model of a launch, in us, fitted to 1,100 times of
+// back-to-back launches on a B200 (17 to 2048 rows, 384 to 8192 columns, K to 8192; within 8 % rms of them; its
+// choice is 1 % slower than the fastest on average, 13 % at most):
+//   few rows: 1.88 + 0.012 bn + (0.107 + 0.0005 bn) k-blocks per CTA, and 0.57 + 0.0035 bn log2(splits) for a
+//     split K (the cluster's barrier and the exchange of partial sums), all clusters running at once;
+//   pairs: 2.95 + (0.9 + 0.277 k-blocks) per round of tiles.
+// E.g. 64 x 4096 x 4096: bn 64 in 4 parts 5.4 us, bn 32 in 2 parts 5.5, bn 64 whole 6.4, pairs 12.5;
+// 1024 x 1024 x 4096: bn 64 whole 6.8 us, bn 128 in 2 parts 7.7, pairs 12.8.
+I8Plan choose_plan(int M, int N, int K, int sms, int dev) {
   const int k_blocks = (K + kBK - 1) / kBK;
   const int64_t ch_tiles = (N - 1) / 128 + 1;
   const int bn2 = N % 256 && N % 192 == 0 ? 192 : 256;
   const int64_t tiles2 = (int64_t(M) + 255) / 256 * ((N - 1) / bn2 + 1);
   I8Plan best{true, bn2, 0};
-  double best_us = 3.9 + 0.28 * k_blocks * static_cast<double>((tiles2 - 1) / (sms / 2) + 1);
+  double best_us = 2.95 + (0.9 + 0.277 * k_blocks) * static_cast<double>((tiles2 - 1) / (sms / 2) + 1);
   for (int bn = 16; bn <= 128; bn *= 2) {
     const int64_t tiles = ch_tiles * ((int64_t(M) + bn - 1) / bn);
-    for (int ls = 0; ls <= 3 && (tiles << ls) <= sms && (1 << ls) <= k_blocks; ++ls) {
-      const double us = 1.65 + 0.0113 * bn + 0.235 * ((k_blocks + (1 << ls) - 1) >> ls) + (ls ? 0.7 + 0.008 * bn * ls : 0);
+    if (tiles > sms) continue;
+    for (int ls = 0; ls <= 3 && (1 << ls) <= k_blocks && tiles <= cluster_room(ls, sms, dev); ++ls) {
+      const int blocks = (k_blocks + (1 << ls) - 1) >> ls;
+      const double us = 1.88 + 0.012 * bn + (0.107 + 0.0005 * bn) * blocks + (ls ? 0.57 + 0.0035 * bn * ls : 0);
       if (us < best_us) {
         best_us = us;
         best = {false, bn, ls};
@@ -1084,8 +1104,9 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   I8Maps maps;
   cudaError_t e;
-  const I8Plan plan = choose_plan(M, N, K, sms);
-  if (few_is_faster(M, N, K)) {
+  const bool few = few_is_faster(M, N, K, sms);
+  const I8Plan plan = few ? I8Plan{} : choose_plan(M, N, K, sms, dev);
+  if (few) {
     e = launch_few_any(A, lda, W, ldw, p, bf16, g, sms, s);
   } else if (!plan.pair) {
     rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
