@@ -582,7 +582,7 @@ def rmsnorm(x, weight=None, eps=1e-6, residual=None, out=None, sum_out=None, str
 
 def rmsnorm_i8(x, weight=None, eps=1e-6, residual=None, sum_out=None, stream=None):
     """rmsnorm with the output in 8 bits: (q int8 [M, D], scale float32 [M]), or (q, scale, v) with a
-    residual; y is q * scale. The rows of q start at multiples of 16 bytes (for linear_i8)."""
+    residual; y is q * scale. The rows of q start at multiples of 16 to 128 bytes (for linear_i8)."""
     if stream is not None:
         with _on(x, stream):
             return rmsnorm_i8(x, weight, eps, residual, sum_out)
@@ -608,7 +608,7 @@ def dequantize_i8(q, scale, dtype=torch.float16, out=None, stream=None):
 
 def linear_i8(A, a_scale, W, w_scale, bias=None, gelu=False, dtype=torch.float16, out=None, stream=None):
     """(A [M, K] @ W [N, K]^T) * a_scale[:, None] * w_scale (+ bias) (+ erf-GELU) in dtype (out's, if given); A, W
-    int8 with rows at multiples of 16 bytes, as quantize_i8 and rmsnorm_i8 return them."""
+    int8 with rows at multiples of 16 bytes (128 is read fastest), as quantize_i8 and rmsnorm_i8 return them."""
     if stream is not None:
         with _on(A, stream):
             return linear_i8(A, a_scale, W, w_scale, bias, gelu, dtype, out)
