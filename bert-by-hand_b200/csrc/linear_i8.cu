@@ -19,6 +19,7 @@
 
 #include <cuda_bf16.h>
 
+#include <cfloat>
 #include <string>
 
 namespace bbh {
@@ -960,6 +961,9 @@ cudaError_t launch_pair_cols(const I8Maps& m, const I8Params& p, bool bf16, bool
 // 89.7. Without GELU eight are as fast at K = 384 (50.5 us for 68451 x 1536) and faster above.
 cudaError_t launch_pair_any(const I8Maps& m, const I8Params& p, int bn, bool bf16, bool gelu, bool tma_c, int dev,
                             int sms, cudaStream_t s) {
+  if (bn == 128)
+    return gelu ? launch_pair_cols<128, 64, true>(m, p, bf16, tma_c, dev, sms, s)
+                : launch_pair_cols<128, 64, false>(m, p, bf16, tma_c, dev, sms, s);
   if (bn == 192)
     return gelu ? launch_pair_cols<192, 64, true>(m, p, bf16, tma_c, dev, sms, s)
                 : launch_pair_cols<192, 64, false>(m, p, bf16, tma_c, dev, sms, s);
@@ -1037,31 +1041,40 @@ int cluster_room(int log_splits, int sms, int dev) {
   return max_clusters(kern, 1 << log_splits, Cfg::THREADS, Cfg::SMEM, sms, room[log_splits], dev);
 }
 
-// The kernel and tile that take the least time by this model of a launch, in us, fitted to 1,100 times of
-// back-to-back launches on a B200 (17 to 2048 rows, 384 to 8192 columns, K to 8192; within 8 % rms of them; its
-// choice is 1 % slower than the fastest on average, 13 % at most):
-//   few rows: 1.88 + 0.012 bn + (0.107 + 0.0005 bn) k-blocks per CTA, and 0.57 + 0.0035 bn log2(splits) for a
-//     split K (the cluster's barrier and the exchange of partial sums), all clusters running at once;
-//   pairs: 2.95 + (0.9 + 0.277 k-blocks) per round of tiles.
-// E.g. 64 x 4096 x 4096: bn 64 in 4 parts 5.4 us, bn 32 in 2 parts 5.5, bn 64 whole 6.4, pairs 12.5;
-// 1024 x 1024 x 4096: bn 64 whole 6.8 us, bn 128 in 2 parts 7.7, pairs 12.8.
-I8Plan choose_plan(int M, int N, int K, int sms, int dev) {
+// The kernel and tile that take the least time by this model of a launch, in us, fitted to 1,700 times of
+// back-to-back launches on a B200 (17 to 68,451 rows, 384 to 8192 columns, K to 8192; within 8 % rms of them; its
+// choice is 1 % slower than the fastest on average, 14 % at most):
+//   few rows: 1.88 + 0.012 bn (with GELU 0.0175) + (0.107 + 0.0005 bn) k-blocks per CTA, and 0.57 + 0.0035 bn
+//     log2(splits) for a split K (the cluster's barrier and the exchange of partial sums), all clusters running
+//     at once;
+//   pairs: a tile's MMAs take k-blocks (0.024 + 0.00103 bn), its epilogue 0.00613 bn - 0.26 (with GELU 0.0115 bn
+//     - 0.23), the longer of them in every round of tiles but one, in which both count; 2.32 a launch, 0.55 a round.
+// E.g. 64 x 4096 x 4096: bn 64 in 4 parts 5.4 us, bn 32 in 2 parts 5.5, bn 64 whole 6.4; 1024 x 1024 x 4096: bn 64
+// whole 6.8 us, bn 128 in 2 parts 7.7, pairs with bn 256 12.8; pairs, 1024 x 4096 x 1024 with GELU: bn 128 7.4 us,
+// 192 8.8, 256 8.5; 4096 x 4096 x 1024 with GELU: 17.1, 16.7, 18.7; 8192 x 4096 x 4096: 91.6, 90.0, 83.4.
+I8Plan choose_plan(int M, int N, int K, bool gelu, int sms, int dev) {
   const int k_blocks = (K + kBK - 1) / kBK;
+  I8Plan best{};
+  double best_us = DBL_MAX;
+  auto consider = [&](double us, const I8Plan& plan) {
+    if (us >= best_us) return;
+    best_us = us;
+    best = plan;
+  };
+  for (int bn = 256; bn >= 128; bn -= 64) {
+    const int64_t tiles = (int64_t(M) + 255) / 256 * ((N - 1) / bn + 1);
+    const double rounds = static_cast<double>((tiles - 1) / (sms / 2) + 1);
+    const double mma = k_blocks * (0.024 + 0.00103 * bn), epi = gelu ? 0.0115 * bn - 0.23 : 0.00613 * bn - 0.26;
+    consider(2.32 + mma + epi + (rounds - 1) * (mma > epi ? mma : epi) + 0.55 * rounds, {true, bn, 0});
+  }
   const int64_t ch_tiles = (N - 1) / 128 + 1;
-  const int bn2 = N % 256 && N % 192 == 0 ? 192 : 256;
-  const int64_t tiles2 = (int64_t(M) + 255) / 256 * ((N - 1) / bn2 + 1);
-  I8Plan best{true, bn2, 0};
-  double best_us = 2.95 + (0.9 + 0.277 * k_blocks) * static_cast<double>((tiles2 - 1) / (sms / 2) + 1);
   for (int bn = 16; bn <= 128; bn *= 2) {
     const int64_t tiles = ch_tiles * ((int64_t(M) + bn - 1) / bn);
     if (tiles > sms) continue;
     for (int ls = 0; ls <= 3 && (1 << ls) <= k_blocks && tiles <= cluster_room(ls, sms, dev); ++ls) {
       const int blocks = (k_blocks + (1 << ls) - 1) >> ls;
-      const double us = 1.88 + 0.012 * bn + (0.107 + 0.0005 * bn) * blocks + (ls ? 0.57 + 0.0035 * bn * ls : 0);
-      if (us < best_us) {
-        best_us = us;
-        best = {false, bn, ls};
-      }
+      consider(1.88 + (gelu ? 0.0175 : 0.012) * bn + (0.107 + 0.0005 * bn) * blocks + (ls ? 0.57 + 0.0035 * bn * ls : 0),
+               {false, bn, ls});
     }
   }
   return best;
@@ -1105,7 +1118,7 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
   I8Maps maps;
   cudaError_t e;
   const bool few = few_is_faster(M, N, K, sms);
-  const I8Plan plan = few ? I8Plan{} : choose_plan(M, N, K, sms, dev);
+  const I8Plan plan = few ? I8Plan{} : choose_plan(M, N, K, g, sms, dev);
   if (few) {
     e = launch_few_any(A, lda, W, ldw, p, bf16, g, sms, s);
   } else if (!plan.pair) {
