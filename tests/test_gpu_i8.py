@@ -339,6 +339,18 @@ def assert_linear(c, a, sa, w, sw, b, dtype):
     assert bool((err <= tol).all()), f"{(err / tol).max().item():.3f} of the tolerance"
 
 
+def assert_linear_gelu(c, a, sa, w, sw, b, dtype):
+    """x Phi(x) = max(x, 0) - |x| Phi(-|x|): Phi(-|x|) is within 5.8e-6 of itself by its fit and 2^-21 by
+    ex2, in all 6.3e-6; the input's error (as without GELU) grows by the GELU's steepest slope, 1.13; two
+    fp32 roundings follow, then the 16-bit one."""
+    p, z = linear64(a, sa, w, sw, b)
+    tail = 0.5 * torch.special.erfc(z.abs() / 2**0.5)
+    want = z.clamp(min=0) - z.abs() * tail
+    tol = 1.13 * U * (2 * p.abs() + z.abs()) + 6.3e-6 * z.abs() * tail + (2 * U + HALF[dtype]) * want.abs() + TINY[dtype]
+    err = (c.double() - want).abs()
+    assert bool((err <= tol * (1 + 1e-6)).all()), f"{(err / tol).max().item():.3f} of the tolerance"
+
+
 LINEAR = [(1, 1, 1), (1, 16, 16), (1, 384, 384), (2, 130, 100), (5, 1000, 31), (16, 128, 128), (17, 127, 129),
           (32, 4096, 1024), (33, 256, 4096), (64, 1152, 384), (65, 1536, 384), (127, 999, 1537), (128, 384, 1536),
           (129, 8, 5000), (200, 257, 640), (1000, 1152, 384), (1024, 1024, 1024), (777, 1001, 333), (3000, 384, 1536),
@@ -362,19 +374,30 @@ def test_linear_i8(M, N, K, dtype):
 @pytest.mark.parametrize("M,N,K", [(3, 200, 96), (64, 384, 384), (300, 513, 384), (3000, 1536, 384), (2500, 1341, 64),
                                    (2600, 1152, 384)])
 def test_linear_i8_gelu(M, N, K, dtype):
-    """x Phi(x) = max(x, 0) - |x| Phi(-|x|): Phi(-|x|) is within 5.8e-6 of itself by its fit and 2^-21 by
-    ex2, in all 6.3e-6; the input's error (as without GELU) grows by the GELU's steepest slope, 1.13; two
-    fp32 roundings follow, then the 16-bit one."""
     import bbh
 
     a, sa, w, sw, b = make_linear(M, N, K, dtype, True)
-    c = bbh.linear_i8(a, sa, w, sw, b, gelu=True, dtype=dtype)
-    p, z = linear64(a, sa, w, sw, b)
-    tail = 0.5 * torch.special.erfc(z.abs() / 2**0.5)
-    want = z.clamp(min=0) - z.abs() * tail
-    tol = 1.13 * U * (2 * p.abs() + z.abs()) + 6.3e-6 * z.abs() * tail + (2 * U + HALF[dtype]) * want.abs() + TINY[dtype]
-    err = (c.double() - want).abs()
-    assert bool((err <= tol * (1 + 1e-6)).all()), f"{(err / tol).max().item():.3f} of the tolerance"
+    assert_linear_gelu(bbh.linear_i8(a, sa, w, sw, b, gelu=True, dtype=dtype), a, sa, w, sw, b, dtype)
+
+
+# one size for each tile and split (on a GPU of 148 SMs): SM pairs with 128, 192 and 256 columns, the last with
+# each number of epilogue warps, stores by TMA or not, and several rounds of tiles; 16 to 128 tokens, K in 1 to 8 parts
+EVERY_KERNEL = [(180, 8304, 65), (161, 8431, 130), (1285, 1680, 200), (556, 6853, 100), (338, 8928, 129), (292, 8235, 90),
+                (2600, 7200, 300), (808, 7200, 1203), (779, 7115, 1233), (3837, 2081, 33), (5000, 4104, 1500),
+                (263, 5104, 100), (2411, 131, 5293), (2598, 142, 5268), (39, 816, 100), (257, 144, 1430), (115, 168, 927),
+                (18, 114, 941), (54, 6464, 100), (18, 4874, 2210), (17, 2256, 1851), (121, 139, 3908), (113, 152, 4890),
+                (3685, 149, 33), (1591, 134, 2975), (1302, 141, 3582), (33, 3192, 3547), (596, 155, 5055)]
+
+
+@pytest.mark.parametrize("M,N,K", EVERY_KERNEL)
+def test_linear_i8_every_kernel(M, N, K):
+    import bbh
+
+    dtype = DTYPES[(M + K) % 2]
+    a, sa, w, sw, b = make_linear(M, N, K, dtype, True)
+    assert_linear(bbh.linear_i8(a, sa, w, sw, b, dtype=dtype), a, sa, w, sw, b, dtype)
+    assert_linear_gelu(bbh.linear_i8(a, sa, w, sw, b, gelu=True, dtype=dtype), a, sa, w, sw, b, dtype)
+    assert bbh.linear_i8_device_error() == 0
 
 
 def test_linear_i8_gelu_over_the_range():
