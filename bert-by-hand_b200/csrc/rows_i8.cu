@@ -219,6 +219,16 @@ __device__ __forceinline__ float steps_per_unit(float top) {
   return r * 127.f * (1.f + 3 * 0x1p-23f);
 }
 
+// 127 / top to half an ulp and a little: one Newton step, for values that do not meet exact halves (kRowNormI8).
+// With the one above, five times further off, ten times as many values of a norm's output were rounded to the
+// other neighbour of a half (about one in 100,000), each of which a layer behind it spreads over its whole row.
+__device__ __forceinline__ float steps_per_unit_near(float top) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
+  const float inv = r * 127.f;
+  return fmaf(fmaf(-inv, top, 127.f), r, inv);
+}
+
 // rint(f * 127 / top) of eight values as bytes: the low byte of f * inv + 1.5 * 2^23, one fma that
 // rounds half to even, with inv from steps_per_unit; f * inv < 127.0001 rounds to 127.
 //
@@ -373,7 +383,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     // that whatever is computed from it is NaN too.
     const bool finite = top <= FLT_MAX;
     const bool zero = !finite || top < 0x1p-120f;
-    const float inv = steps_per_unit(zero ? 1.f : top);
+    const float inv = MODE == kRowQuant ? steps_per_unit(zero ? 1.f : top) : steps_per_unit_near(zero ? 1.f : top);
     bool ties = false;
     float rest = 0.f;
     if constexpr (MODE == kRowQuant) {
