@@ -9,7 +9,10 @@
 // rstd cancels out of q (q = rint(v w * 127 / max|v w|), scale = max|v w| * rstd / 127), so the
 // sum of squares and the maximum are reduced together, with one exchange between the warps
 // of a row. All arithmetic is fp32; the only roundings are those of the outputs.
-// Bound: HBM bytes (x, residual, sum, y or q; each moved once).
+// Bound: HBM bytes (x, residual, sum, y or q; each moved once). On a B200 whose copies reach 6.5 TB/s:
+// 8192 x 4096 bf16 with a residual rmsnorm 41.2 us = 6.5 TB/s, rmsnorm_i8 37.2 = 6.3; without rmsnorm 22.0 = 6.1,
+// rmsnorm_i8 21.4 = 4.7 (its arithmetic per byte is twice that with one); quantize_i8 16.9 = 6.0, dequantize_i8
+// 15.0 = 6.7; 20000 x 1023 fp16 rmsnorm 16.2 = 5.0.
 #include "common.cuh"
 #include "internal.h"
 #include "../../include/bbh.h"
@@ -39,7 +42,7 @@ struct RowParams {
 };
 
 constexpr int kRowBlock = 128;  // threads of a block when a row takes fewer
-constexpr int kRowMaxBlock = 512;  // leaves 128 registers a thread: no spills at any width
+constexpr int kRowMaxBlock = 512;  // leaves 128 registers a thread (only 2-byte accesses at the widest spill some)
 
 template <bool BF16>
 __device__ __forceinline__ float2 unpack16(uint32_t w) {
@@ -281,41 +284,46 @@ __device__ __forceinline__ void group_reduce(float& s, float& m, int group) {
 }
 
 // V: 8-element chunks a thread holds. 64 registers up to four chunks (32 warps an SM: with 82, norm of
-// 8192 x 4096 took 27.1 us instead of 22.9).
-template <int MODE, bool BF16, int V, int CUT>
+// 8192 x 4096 took 27.1 us instead of 22.9). RES: with a residual (a kernel of its own: without one 16384 x 1536
+// rmsnorm takes 16.4 us instead of 17.4, 20000 x 1023 16.3 instead of 17.5). Where little is done to an element
+// its packed form is kept and unpacked twice (16384 x 1536 rmsnorm 16.1; rmsnorm_i8, which would need
+// the weight twice as well, 17.9 instead of 15.2).
+template <int MODE, bool BF16, int V, int CUT, bool RES>
 __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1) row_kernel(const RowParams p) {
+  // whether the row stays packed in registers and is unpacked a second time for the output
+  constexpr bool kTwice = MODE == kRowQuant || (MODE == kRowNorm && !RES);
   pdl_launch_dependents();
   const int group = p.group;
   const int t = threadIdx.x & (group - 1);
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
   const bool live = r < p.rows;
   const uint16_t* x = p.x + r * p.ldx;
-  const uint16_t* residual = MODE != kRowQuant && p.residual ? p.residual + r * p.ldr : nullptr;
+  const uint16_t* residual = RES ? p.residual + r * p.ldr : nullptr;
   const uint16_t* weight = MODE != kRowQuant ? p.weight : nullptr;
   uint16_t* sum = p.sum + r * p.lds;
   const Place at = place<CUT>(x, t, group, live ? p.D : 0);  // a group behind the last row has no elements
   const bool edge = CUT == kShifted && at.edge >= 0;
   pdl_wait();
 
-  uint4 ux[V], ur[V];
+  uint4 ux[V], ur[RES ? V : 1];
 #pragma unroll
   for (int j = 0; j < V; ++j) ux[j] = load8<CUT>(x, at, j);
-  if (residual) {
+  if constexpr (RES) {
 #pragma unroll
     for (int j = 0; j < V; ++j) ur[j] = load8<CUT>(residual, at, j);
   }
   float fe = 0.f;  // the edge element
   if (edge) {
     fe = load1<BF16>(x, at.edge);
-    if (residual) fe += load1<BF16>(residual, at.edge);
+    if constexpr (RES) fe += load1<BF16>(residual, at.edge);
   }
 
-  float f[8 * V];
+  float f[kTwice ? 8 : 8 * V];
   float ss = 0.f, ss1 = 0.f, top = 0.f;
   uint32_t top2 = 0;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    float* v = f + 8 * j;
+    float* v = kTwice ? f : f + 8 * j;
     if constexpr (MODE == kRowQuant) {  // the packed values are enough until the scale is known
       top2 = max_abs_nan2<BF16>(top2, ux[j].x);
       top2 = max_abs_nan2<BF16>(top2, ux[j].y);
@@ -323,7 +331,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
       top2 = max_abs_nan2<BF16>(top2, ux[j].w);
     } else {
       unpack8<BF16>(ux[j], v);
-      if (residual) {
+      if constexpr (RES) {
         float u[8];
         unpack8<BF16>(ur[j], u);
 #pragma unroll
@@ -352,7 +360,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     top = max_nan(m.x, m.y);
   }
   if (edge) {
-    if (residual && p.sum) store1<BF16>(sum, at.edge, fe);
+    if (RES && p.sum) store1<BF16>(sum, at.edge, fe);
     ss1 = fmaf(fe, fe, ss1);
     if (weight) fe *= load1<BF16>(weight, at.edge);
     top = max_abs_nan(top, fe, 0.f);
@@ -361,11 +369,18 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
   group_reduce<MODE != kRowQuant, MODE != kRowNorm>(ss, top, group);
   const float rstd = MODE == kRowQuant ? 1.f : rsqrtf(ss * p.inv_D + p.eps);
 
+  // the packed values again: they take half the registers, and the compiler shall not keep the others
+  auto again = [&](int j) {
+    uint4 u = ux[j];
+    asm volatile("" : "+r"(u.x), "+r"(u.y), "+r"(u.z), "+r"(u.w));
+    unpack8<BF16>(u, f);
+  };
   if constexpr (MODE == kRowNorm) {
     uint16_t* y = p.y + r * p.ldy;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float* v = f + 8 * j;
+      float* v = kTwice ? f : f + 8 * j;
+      if (kTwice) again(j);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= rstd;
       if (weight) {
@@ -400,8 +415,8 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
       const int sh = -at.head & 7, first = sh ? 1 : 0;  // the piece of chunk 0
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (MODE == kRowQuant) unpack8<BF16>(ux[j], f + 8 * j);
-        if (chunk_at<CUT>(at, j) >= 0) row[first + j * group + t] = quantize8(f + 8 * j, inv, rest, ties);
+        if (kTwice) again(j);
+        if (chunk_at<CUT>(at, j) >= 0) row[first + j * group + t] = quantize8(kTwice ? f : f + 8 * j, inv, rest, ties);
       }
       if (edge) reinterpret_cast<uint8_t*>(row)[at.edge + sh] = quantize1(fe, inv, rest, ties);
       __syncthreads();
@@ -419,8 +434,8 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (MODE == kRowQuant) unpack8<BF16>(ux[j], f + 8 * j);
-        uint2 o = quantize8(f + 8 * j, inv, rest, ties);
+        if (kTwice) again(j);
+        uint2 o = quantize8(kTwice ? f : f + 8 * j, inv, rest, ties);
         if (zero) o = make_uint2(0, 0);
         if constexpr (CUT == kAligned) {
           const int e = chunk_at<CUT>(at, j);
@@ -519,7 +534,7 @@ int row_group(int rows, int D, int num_sms, int* chunks) {
   return g;
 }
 
-template <int MODE, bool BF16, int CUT>
+template <int MODE, bool BF16, int CUT, bool RES>
 cudaError_t launch_rows(const RowParams& p, int chunks, cudaStream_t s) {
   const int block = p.group < kRowBlock ? kRowBlock : p.group;
   const int per = block / p.group;
@@ -529,23 +544,30 @@ cudaError_t launch_rows(const RowParams& p, int chunks, cudaStream_t s) {
     return launch_ex(kern, grid, dim3(block), smem, s, true, 1, p);
   };
   switch (chunks) {
-    case 1: return go(row_kernel<MODE, BF16, 1, CUT>, 1);
-    case 2: return go(row_kernel<MODE, BF16, 2, CUT>, 2);
-    case 3: return go(row_kernel<MODE, BF16, 3, CUT>, 3);
-    case 4: return go(row_kernel<MODE, BF16, 4, CUT>, 4);
-    default: return go(row_kernel<MODE, BF16, 8, CUT>, 8);
+    case 1: return go(row_kernel<MODE, BF16, 1, CUT, RES>, 1);
+    case 2: return go(row_kernel<MODE, BF16, 2, CUT, RES>, 2);
+    case 3: return go(row_kernel<MODE, BF16, 3, CUT, RES>, 3);
+    case 4: return go(row_kernel<MODE, BF16, 4, CUT, RES>, 4);
+    default: return go(row_kernel<MODE, BF16, 8, CUT, RES>, 8);
   }
+}
+
+template <int MODE, bool BF16, int CUT>
+cudaError_t launch_cut(const RowParams& p, int chunks, cudaStream_t s) {
+  if constexpr (MODE != kRowQuant)
+    if (p.residual) return launch_rows<MODE, BF16, CUT, true>(p, chunks, s);
+  return launch_rows<MODE, BF16, CUT, false>(p, chunks, s);
 }
 
 template <int MODE>
 cudaError_t launch_mode(const RowParams& p, bool bf16, Cut cut, int chunks, cudaStream_t s) {
   switch (cut) {
     case kAligned:
-      return bf16 ? launch_rows<MODE, true, kAligned>(p, chunks, s) : launch_rows<MODE, false, kAligned>(p, chunks, s);
+      return bf16 ? launch_cut<MODE, true, kAligned>(p, chunks, s) : launch_cut<MODE, false, kAligned>(p, chunks, s);
     case kShifted:
-      return bf16 ? launch_rows<MODE, true, kShifted>(p, chunks, s) : launch_rows<MODE, false, kShifted>(p, chunks, s);
+      return bf16 ? launch_cut<MODE, true, kShifted>(p, chunks, s) : launch_cut<MODE, false, kShifted>(p, chunks, s);
     default:
-      return bf16 ? launch_rows<MODE, true, kSingle>(p, chunks, s) : launch_rows<MODE, false, kSingle>(p, chunks, s);
+      return bf16 ? launch_cut<MODE, true, kSingle>(p, chunks, s) : launch_cut<MODE, false, kSingle>(p, chunks, s);
   }
 }
 
