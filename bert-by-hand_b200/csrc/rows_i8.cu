@@ -523,13 +523,17 @@ namespace {
 
 // Threads of a row and 8-element chunks a thread: the smallest power of two that leaves at
 // most four chunks a thread (eight in rows of more than 16,384 elements); with few rows, more threads
-// a row (down to one chunk each), since the chip then waits on one row's loads and not on bandwidth.
+// a row (down to one chunk each), since the chip then waits on one row's loads and not on bandwidth:
+// up to two rows an SM, and the norms, which have more to do, until there are 512 threads an SM
+// (rmsnorm_i8 with a residual, 1024 x 1024: 3.2 us instead of 3.6, 2048 x 1024 3.8 / 4.5, 1000 x 1023 3.9 / 5.6;
+// quantize_i8 of 1000 x 1023 would take 3.4 instead of 2.7).
 // Two chunks instead of four at many rows: 8192 x 4096 rmsnorm_i8 22.7 -> 31.1 us.
-int row_group(int rows, int D, int num_sms, int* chunks) {
+int row_group(int rows, int D, int num_sms, bool norm, int* chunks) {
   const int n = (D + 7) / 8;
   int g = 16;
   while (g < kRowMaxBlock && (n + g - 1) / g > 4) g *= 2;
-  while (rows <= 2 * num_sms && g < kRowMaxBlock && (n + g - 1) / g > 1) g *= 2;
+  auto few = [&] { return rows <= 2 * num_sms || (norm && int64_t(rows) * g < int64_t(512) * num_sms); };
+  while (few() && g < kRowMaxBlock && (n + g - 1) / g > 1) g *= 2;
   *chunks = (n + g - 1) / g;
   return g;
 }
@@ -633,7 +637,7 @@ int run_rows(const char* who, int mode, RowParams p, int dtype, void* stream) {
   aligned = aligned && shifted;
   const Cut cut = aligned ? kAligned : shifted ? kShifted : kSingle;
   int chunks = 0;
-  p.group = row_group(p.rows, p.D, sms, &chunks);
+  p.group = row_group(p.rows, p.D, sms, mode != kRowQuant, &chunks);
   p.inv_D = 1.0f / static_cast<float>(p.D);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == BBH_BF16;
@@ -688,7 +692,7 @@ int bbh_dequantize_i8(const int8_t* q, int64_t ldq, const float* scale, uint16_t
   const bool q8 = !off(q, 8) && ldq % 8 == 0;
   const Cut cut = q8 && D % 8 == 0 && !off(y, 16) && ldy % 8 == 0 ? kAligned : q8 ? kShifted : kSingle;
   int chunks = 0;
-  DequantParams p{q, scale, y, ldq, ldy, M, D, row_group(M, D, sms, &chunks)};
+  DequantParams p{q, scale, y, ldq, ldy, M, D, row_group(M, D, sms, false, &chunks)};
   const int block = p.group < kRowBlock ? kRowBlock : p.group;
   const int per = block / p.group;
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(M) + per - 1) / per));
