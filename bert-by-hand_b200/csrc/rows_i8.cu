@@ -11,9 +11,10 @@
 // of a row. All arithmetic is fp32; the only roundings are those of the outputs.
 // Bound: HBM bytes (x, residual, sum, y or q; each moved once). On a B200 whose copies reach 6.5 TB/s:
 // 8192 x 4096 bf16 with a residual rmsnorm 41.2 us = 6.5 TB/s, rmsnorm_i8 37.2 = 6.3; without rmsnorm 22.0 = 6.1,
-// rmsnorm_i8 21.4 = 4.7 (its arithmetic per byte is twice that with one); quantize_i8 16.9 = 6.0, dequantize_i8
-// 15.0 = 6.7; 20000 x 1023 fp16 rmsnorm 16.2 = 5.0.
+// rmsnorm_i8 20.4 = 4.9 (its arithmetic per byte is twice that with one); quantize_i8 16.9 = 6.0, dequantize_i8
+// 15.0 = 6.7; 20000 x 1023 fp16 rmsnorm 15.8 = 5.2.
 #include "common.cuh"
+#include "epilogue.cuh"
 #include "internal.h"
 #include "../../include/bbh.h"
 
@@ -208,6 +209,26 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
                     pack16<BF16>(f[6], f[7]));
 }
 
+// v *= u, and ss += v[even]^2, ss1 += v[odd]^2, of eight values in packed pairs: half the instructions
+// (8192 x 4096 rmsnorm_i8 20.4 us instead of 21.4).
+__device__ __forceinline__ void mul8(float* v, const float* u) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 z = f2_split(f2_mul(f2(v[i], v[i + 1]), f2(u[i], u[i + 1])));
+    v[i] = z.x;
+    v[i + 1] = z.y;
+  }
+}
+__device__ __forceinline__ void squares8(const float* v, float& ss, float& ss1) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const unsigned long long z = f2(v[i], v[i + 1]);
+    const float2 t = f2_split(f2_fma(z, z, f2(ss, ss1)));
+    ss = t.x;
+    ss1 = t.y;
+  }
+}
+
 // The low bytes of eight words.
 __device__ __forceinline__ uint2 low_bytes(const uint32_t* b) {
   return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
@@ -240,9 +261,18 @@ __device__ __forceinline__ float steps_per_unit_near(float top) {
 // above, takes it to 64, the even neighbour; with 11-bit significands every other value is at least
 // 2^-20 of itself away from a half, more than inv is off. If 127 divides it (`ties`), f * inv + f * rest,
 // with rest what inv lacks of 127 / top, is right to fp32 and a half stays one.
+// HALVES: whether exact halves occur (kRowQuant; without, packed pairs are faster, with them slower).
+template <bool HALVES>
 __device__ __forceinline__ uint2 quantize8(const float* f, float inv, float rest, bool ties) {
   uint32_t b[8];
-  if (ties) {
+  if constexpr (!HALVES) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float2 z = f2_split(f2_fma(f2(f[i], f[i + 1]), f2(inv, inv), f2(12582912.f, 12582912.f)));
+      b[i] = __float_as_uint(z.x);
+      b[i + 1] = __float_as_uint(z.y);
+    }
+  } else if (ties) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(fmaf(f[i], inv, f[i] * rest) + 12582912.f);
   } else {
@@ -338,18 +368,13 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
         for (int i = 0; i < 8; ++i) v[i] += u[i];
         if (p.sum) store8<CUT>(sum, at, j, pack8<BF16>(v));
       }
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        ss = fmaf(v[i], v[i], ss);
-        ss1 = fmaf(v[i + 1], v[i + 1], ss1);
-      }
+      squares8(v, ss, ss1);
     }
     if constexpr (MODE == kRowNormI8) {
       if (weight) {
         float u[8];
         unpack8<BF16>(load_weight8<CUT>(weight, at, j), u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= u[i];
+        mul8(v, u);
       }
 #pragma unroll
       for (int i = 0; i < 8; i += 2) top = max_abs_nan(top, v[i], v[i + 1]);
@@ -386,8 +411,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
       if (weight) {
         float u[8];
         unpack8<BF16>(load_weight8<CUT>(weight, at, j), u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= u[i];
+        mul8(v, u);
       }
       store8<CUT>(y, at, j, pack8<BF16>(v));
     }
@@ -416,7 +440,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if (kTwice) again(j);
-        if (chunk_at<CUT>(at, j) >= 0) row[first + j * group + t] = quantize8(kTwice ? f : f + 8 * j, inv, rest, ties);
+        if (chunk_at<CUT>(at, j) >= 0) row[first + j * group + t] = quantize8<MODE == kRowQuant>(kTwice ? f : f + 8 * j, inv, rest, ties);
       }
       if (edge) reinterpret_cast<uint8_t*>(row)[at.edge + sh] = quantize1(fe, inv, rest, ties);
       __syncthreads();
@@ -435,7 +459,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if (kTwice) again(j);
-        uint2 o = quantize8(kTwice ? f : f + 8 * j, inv, rest, ties);
+        uint2 o = quantize8<MODE == kRowQuant>(kTwice ? f : f + 8 * j, inv, rest, ties);
         if (zero) o = make_uint2(0, 0);
         if constexpr (CUT == kAligned) {
           const int e = chunk_at<CUT>(at, j);
