@@ -31,7 +31,18 @@ struct I8Params {
   uint16_t* C;
   int64_t ldc;
   int M, N, K;
+  const int8_t* W;  // few rows: to L2 while the kernel in front still runs (see kPrefetchBytes), else null
+  int64_t ldw;
 };
+
+// Weights are constants of a model and, one token after the other, come from HBM: the kernels for few rows ask
+// for theirs before they wait for the kernel in front of them. That brings bytes to L2 and reads none, so what
+// that kernel may still write to W is seen after the wait. 16 pairs of quantize_i8 and linear_i8 with weights of
+// 4096 x 4096 each, one token: 106 -> 96 us; 16 tokens 119 -> 107, 64 tokens 143 -> 137. Where the weights are in
+// L2 already it costs 0 to 0.2 us a launch; with much more of them than L2 takes it only changes the order of
+// the reads (16384 x 4096: 12.4 -> 13.4 us).
+constexpr int64_t kPrefetchBytes = int64_t(32) << 20;
+constexpr int kPrefetchBlocks = 4;  // k-blocks of a CTA, few-rows kernel (all of them: twice the loss, little more gain)
 
 __device__ int g_i8_err;  // first device error of these kernels (kDevWaitTimeout)
 
@@ -82,6 +93,11 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
+}
+
+// `bytes` (a multiple of 16, at a multiple of 16) to L2.
+__device__ __forceinline__ void l2_prefetch(const void* at, uint32_t bytes) {
+  if (bytes) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(bytes) : "memory");
 }
 
 // Instruction descriptor, kind::i8: signed A and B, int32 D, both K-major.
@@ -604,6 +620,13 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  if (p.W && blockIdx.y == 0 && warp >= 2 && warp < 6) {  // not by TMA, which takes its orders one after the other
+    const int row = n0 + static_cast<int>(threadIdx.x) - 64;
+    if (row < p.N) {
+      for (int kb = kb0; kb < min(kb1, kb0 + kPrefetchBlocks); ++kb)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.W + row * p.ldw + kb * kBK));
+    }
+  }
   pdl_wait();
   if (log_splits) cluster_arrive_relaxed();  // this CTA runs: its shared memory may be written (waited for below)
 
@@ -796,7 +819,7 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
 // barriers, a cluster) are as long as their transfer. So no staging: a CTA has 16 output channels, its
 // eight warps every eighth 64 bytes of K, loaded straight into the fragments of mma.sync m16n8k32 (the
 // order of k is free as long as both operands have the same, so a lane's 16 consecutive bytes are four
-// of its fragments' words), and the partial sums meet in shared memory. 1 x 4096 x 4096: 3.2 us = 5.2 TB/s
+// of its fragments' words), and the partial sums meet in shared memory. 1 x 4096 x 4096: 3.3 us = 5.1 TB/s
 // of weights (they fit in L2 when repeated), 1 x 8192 x 8192 8.2 us = 8.2 TB/s.
 constexpr int kFewWarps = 8;
 
@@ -844,6 +867,7 @@ __global__ void __launch_bounds__(32 * kFewWarps)
 #pragma unroll
   for (int t = 0; t < MT; ++t) x[t] = A + static_cast<int64_t>(min(8 * t + g, p.M - 1)) * lda;
   int acc[MT][4] = {};
+  if (p.W && threadIdx.x < 16 && n0 + threadIdx.x < p.N) l2_prefetch(W + (n0 + threadIdx.x) * ldw, p.K & ~15);
   pdl_wait();
   for (int k0 = 64 * warp; k0 < p.K; k0 += 64 * kFewWarps * U) {
     uint4 a[U], b[U], v[U][MT];
@@ -1013,12 +1037,13 @@ cudaError_t launch_few_any(const int8_t* A, int64_t lda, const int8_t* W, int64_
                      : launch_few<1, 8>(A, lda, W, ldw, p, bf16, gelu, s);
 }
 
-// Whether that kernel takes less time than the tcgen05 one (us, few rows / tcgen05): 1 x 4096 x 4096 3.3 / 4.1;
-// 1 x 2048 x 8192 4.7 / 4.4; 4 x 16384 x 4096 8.8 / 8.7; 8 x 4096 x 4096 3.6 / 4.0; 8 x 16384 x 4096 9.5 / 7.3;
-// 16 x 1536 x 384 2.3 / 2.3; 16 x 1024 x 1024 2.1 / 2.9; 16 x 1024 x 4096 3.8 / 3.3; 16 x 4096 x 4096 5.6 / 4.0.
+// Whether that kernel takes less time than the tcgen05 one (us, few rows / tcgen05), with the weights in L2: 1 x 4096
+// x 4096 3.3 / 4.1; 1 x 2048 x 8192 4.7 / 4.4; 4 x 16384 x 4096 8.8 / 8.7; 8 x 4096 x 4096 3.6 / 4.0; 8 x 16384 x
+// 4096 9.5 / 7.3; 16 x 1536 x 384 2.3 / 2.3; 16 x 1024 x 1024 2.1 / 2.9; 16 x 1024 x 4096 3.8 / 3.3; 16 x 4096 x 4096
+// 5.6 / 4.0; and in HBM: 1 x 4096 x 4096 4.5 / 5.2; 1 x 8192 x 2048 4.5 / 5.0; 1 x 16384 x 4096 13.9 / 12.4.
 bool few_is_faster(int M, int N, int K, int sms) {
   const int64_t weights = int64_t(N) * K;
-  if (M <= 8) return (M <= 4 || weights <= (int64_t(16) << 20)) && (K <= 4096 || N > 16 * sms);
+  if (M <= 8) return weights <= (int64_t(16) << 20) && (K <= 4096 || N > 16 * sms);
   return M <= 16 && K <= 2048 && weights <= (int64_t(4) << 20);
 }
 
@@ -1110,7 +1135,7 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
   int rc = unit_device(&dev, &sms);
   if (rc) return rc;
 
-  I8Params p{a_scale, w_scale, bias, C, ldc, M, N, K};
+  I8Params p{a_scale, w_scale, bias, C, ldc, M, N, K, int64_t(N) * K <= kPrefetchBytes ? W : nullptr, ldw};
   const bool bf16 = dtype == BBH_BF16, g = gelu != 0;
   // N % 8: a TMA store ends at a 16-byte boundary, not inside one (it overwrote up to 7 elements of padding)
   const bool tma_c = !(bits(C) & 15) && ldc % 8 == 0 && N % 8 == 0;

@@ -595,6 +595,30 @@ def test_captured_and_replayed(M):
             assert torch.equal(y, y0) and torch.equal(v, v0)
 
 
+@pytest.mark.parametrize("M", [1, 24, 200])
+def test_weights_written_by_the_kernel_in_front(M):
+    """Weights that the call before has just quantised, into the same memory every time: a launch that starts
+    early must not see the old ones."""
+    import bbh
+
+    N, K, rounds = 1024, 2048, 40
+    g = gen("rewritten", M)
+    ws = rows16(rounds * N, K, torch.float16, g).view(rounds, N, K)
+    a, sa = int8_rows(M, K, g), torch.rand(M, generator=g, device=DEV)
+    outs = torch.empty(rounds, M, N, dtype=torch.float16, device=DEV)
+    pointers = set()
+    for i in range(rounds):
+        wq, s = bbh.quantize_i8(ws[i])
+        bbh.linear_i8(a, sa, wq, s, out=outs[i])
+        pointers.add(wq.data_ptr())
+        del wq, s
+    assert len(pointers) <= 2
+    for i in range(rounds):
+        wq, s = bbh.quantize_i8(ws[i])
+        torch.cuda.synchronize()
+        assert torch.equal(bbh.linear_i8(a, sa, wq, s), outs[i])
+
+
 _FIRST_CALLS = """
 import sys
 sys.path[:0] = [{here!r}]
