@@ -27,20 +27,20 @@ namespace bbh {
 
 enum RowMode : int { kRowNorm = 0, kRowNormI8 = 1, kRowQuant = 2 };
 
-struct RowParams {
+struct RowParams {  // 96 bytes: above, a launch takes the host 0.35 us longer
   const uint16_t* x;
   const uint16_t* residual;  // null: none
   const uint16_t* weight;    // null: ones
-  uint16_t* y;               // kRowNorm
-  int8_t* q;                 // 8-bit modes
+  void* out;                 // kRowNorm: 16-bit, else int8
   float* scale;              // 8-bit modes
   uint16_t* sum;             // written when residual is given and sum is not null
-  int64_t ldx, ldr, ldy, ldq, lds;
+  int64_t ldx, ldr, ldo, lds;
   int rows, D;
   int group;  // threads of a row: a power of two, 16 .. 512
   float eps;
-  float inv_D;  // 1 / D
 };
+
+static_assert(sizeof(RowParams) == 96, "kernel arguments");
 
 constexpr int kRowBlock = 128;  // threads of a block when a row takes fewer
 constexpr int kRowMaxBlock = 512;  // leaves 128 registers a thread (only 2-byte accesses at the widest spill some)
@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
   uint16_t* sum = p.sum + r * p.lds;
   const Place at = place<CUT>(x, t, group, live ? p.D : 0);  // a group behind the last row has no elements
   const bool edge = CUT == kShifted && at.edge >= 0;
+  const float inv_D = MODE == kRowQuant ? 0.f : __frcp_rn(static_cast<float>(p.D));
   pdl_wait();
 
   uint4 ux[V], ur[RES ? V : 1];
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
   }
   ss += ss1;
   group_reduce<MODE != kRowQuant, MODE != kRowNorm>(ss, top, group);
-  const float rstd = MODE == kRowQuant ? 1.f : rsqrtf(ss * p.inv_D + p.eps);
+  const float rstd = MODE == kRowQuant ? 1.f : rsqrtf(ss * inv_D + p.eps);
 
   // the packed values again: they take half the registers, and the compiler shall not keep the others
   auto again = [&](int j) {
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     unpack8<BF16>(u, f);
   };
   if constexpr (MODE == kRowNorm) {
-    uint16_t* y = p.y + r * p.ldy;
+    uint16_t* y = static_cast<uint16_t*>(p.out) + r * p.ldo;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float* v = kTwice ? f : f + 8 * j;
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
       if (ties) rest = fmaf(-inv, top, 127.f) / top;
     }
     if (live && t == 0) p.scale[r] = !finite ? __int_as_float(0x7fc00000) : zero ? 0.f : top / 127.f * rstd;
-    int8_t* q = p.q + r * p.ldq;
+    int8_t* q = static_cast<int8_t*>(p.out) + r * p.ldo;
     if constexpr (CUT == kShifted) {
       // The bytes of a chunk are not where an aligned store of q wants them: through shared memory, element e
       // at byte e + sh, so that chunks are 8-byte pieces there. The rows of q are 8-byte aligned.
@@ -622,15 +623,15 @@ int run_rows(const char* who, int mode, RowParams p, int dtype, void* stream) {
   if (rc) return rc;
   if (p.rows == 0) return BBH_OK;
   const bool i8 = mode != kRowNorm;
-  if (!p.x || (i8 ? (!p.q || !p.scale) : !p.y)) return internal_fail(BBH_ERR_ARG, w + ": null pointer");
+  if (!p.x || !p.out || (i8 && !p.scale)) return internal_fail(BBH_ERR_ARG, w + ": null pointer");
   if (p.sum && !p.residual) return internal_fail(BBH_ERR_ARG, w + ": sum needs a residual");
   if (!(p.eps >= 0.f) || p.eps > FLT_MAX) return internal_fail(BBH_ERR_ARG, w + ": eps must be finite and >= 0");
-  if (p.ldx < p.D || (p.residual && p.ldr < p.D) || (p.sum && p.lds < p.D) || (i8 ? p.ldq < p.D : p.ldy < p.D))
+  if (p.ldx < p.D || (p.residual && p.ldr < p.D) || (p.sum && p.lds < p.D) || p.ldo < p.D)
     return internal_fail(BBH_ERR_ARG, w + ": a row stride is smaller than D");
-  if (off(p.x, 2) || off(p.residual, 2) || off(p.weight, 2) || off(p.sum, 2) || off(p.y, 2) || off(p.scale, 4))
+  if (off(p.x, 2) || off(p.residual, 2) || off(p.weight, 2) || off(p.sum, 2) || (!i8 && off(p.out, 2)) || off(p.scale, 4))
     return internal_fail(BBH_ERR_ARG, w + ": a pointer is not aligned to its elements");
-  const void* outs[3] = {i8 ? static_cast<void*>(p.q) : p.y, p.sum, p.scale};
-  const Span so[3] = {i8 ? span(p.q, p.ldq, p.rows, p.D, 1) : span(p.y, p.ldy, p.rows, p.D, 2),
+  const void* outs[3] = {p.out, p.sum, p.scale};
+  const Span so[3] = {span(p.out, p.ldo, p.rows, p.D, i8 ? 1 : 2),
                       span(p.sum, p.lds, p.rows, p.D, 2), span(p.scale, 1, p.rows, 1, 4)};
   const void* ins[3] = {p.x, p.residual, p.weight};
   const Span si[3] = {span(p.x, p.ldx, p.rows, p.D, 2), span(p.residual, p.ldr, p.rows, p.D, 2),
@@ -647,7 +648,7 @@ int run_rows(const char* who, int mode, RowParams p, int dtype, void* stream) {
   rc = unit_device(&dev, &sms);
   if (rc) return rc;
   // the cut that the operands allow (see Cut)
-  bool aligned = p.D % 8 == 0, shifted = !off(p.weight, 16) && (!i8 || (!off(p.q, 8) && p.ldq % 8 == 0));
+  bool aligned = p.D % 8 == 0, shifted = !off(p.weight, 16) && (!i8 || (!off(p.out, 8) && p.ldo % 8 == 0));
   auto look = [&](const uint16_t* q, int64_t ld) {
     if (!q) return;
     aligned = aligned && !off(q, 16) && ld % 8 == 0;
@@ -657,12 +658,11 @@ int run_rows(const char* who, int mode, RowParams p, int dtype, void* stream) {
   look(p.x, p.ldx);
   look(p.residual, p.ldr);
   look(p.sum, p.lds);
-  look(p.y, p.ldy);
+  if (!i8) look(static_cast<const uint16_t*>(p.out), p.ldo);
   aligned = aligned && shifted;
   const Cut cut = aligned ? kAligned : shifted ? kShifted : kSingle;
   int chunks = 0;
   p.group = row_group(p.rows, p.D, sms, mode != kRowQuant, &chunks);
-  p.inv_D = 1.0f / static_cast<float>(p.D);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == BBH_BF16;
   const cudaError_t e = mode == kRowNorm     ? launch_mode<kRowNorm>(p, bf, cut, chunks, s)
@@ -680,20 +680,20 @@ extern "C" {
 int bbh_rmsnorm(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr, const uint16_t* weight,
                 uint16_t* y, int64_t ldy, uint16_t* sum, int64_t lds, int M, int D, float eps, int dtype,
                 void* stream) {
-  bbh::RowParams p{x, residual, weight, y, nullptr, nullptr, sum, ldx, ldr, ldy, 0, lds, M, D, 0, eps, 0.f};
+  bbh::RowParams p{x, residual, weight, y, nullptr, sum, ldx, ldr, ldy, lds, M, D, 0, eps};
   return bbh::run_rows("bbh_rmsnorm", bbh::kRowNorm, p, dtype, stream);
 }
 
 int bbh_rmsnorm_i8(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr, const uint16_t* weight,
                    int8_t* q, int64_t ldq, float* scale, uint16_t* sum, int64_t lds, int M, int D, float eps,
                    int dtype, void* stream) {
-  bbh::RowParams p{x, residual, weight, nullptr, q, scale, sum, ldx, ldr, 0, ldq, lds, M, D, 0, eps, 0.f};
+  bbh::RowParams p{x, residual, weight, q, scale, sum, ldx, ldr, ldq, lds, M, D, 0, eps};
   return bbh::run_rows("bbh_rmsnorm_i8", bbh::kRowNormI8, p, dtype, stream);
 }
 
 int bbh_quantize_i8(const uint16_t* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int M, int D, int dtype,
                     void* stream) {
-  bbh::RowParams p{x, nullptr, nullptr, nullptr, q, scale, nullptr, ldx, 0, 0, ldq, 0, M, D, 0, 0.f, 0.f};
+  bbh::RowParams p{x, nullptr, nullptr, q, scale, nullptr, ldx, 0, ldq, 0, M, D, 0, 0.f};
   return bbh::run_rows("bbh_quantize_i8", bbh::kRowQuant, p, dtype, stream);
 }
 
