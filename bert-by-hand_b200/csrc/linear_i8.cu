@@ -116,33 +116,38 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // erf-GELU, x Phi(x) = max(x, 0) - |x| Phi(-|x|), of N pairs of fp32 values side by side (which hides
-// the fmas' latency). log2 Phi(-a) is close to a parabola and is evaluated as a polynomial of degree 7
+// the fmas' latency). log2 Phi(-a) is close to a parabola and is evaluated as a polynomial of degree 10
 // in a (this project's own least-squares fit on [0, 5.75], weighted by what an error means to the
-// output and reweighted to equal ripple): Phi(-a) is within 5.8e-6 of itself there (2.2e-6 rms);
-// beyond, the polynomial keeps falling, and Phi with it, so no clamp is needed. The output is within
-// 1e-6 max(|x|, 1), far inside its 16-bit rounding.
+// output and reweighted to equal ripple): Phi(-a) is within 1.8e-7 of itself up to a = 4, 2e-6 up to 5.75;
+// beyond, the polynomial keeps falling, and Phi with it, so no clamp is needed. With the roundings of the
+// sum and of ex2 the output is within 1e-7 max(|x|, 1).
+// Why this degree: of normal x 0.009 % of the fp16 outputs are the other neighbour of the exact value, 0.018 %
+// with fp32's erf. Degree 7 (Phi within 5.8e-6) has 0.20 %, and a quantiser behind the layer then rounds ten times
+// as many of its integers the other way, each of which the next layer spreads over a row; degree 9 0.018 to
+// 0.03 %. 68451 x 1536 x 384: 68.9 us with degree 7 one value at a time, here, in packed pairs (half the
+// issue slots), 73.8; degree 9 71.8; degree 10 one value at a time 82.3.
 template <int N>
 __device__ __forceinline__ void gelu2(unsigned long long (&x)[N]) {
-  constexpr float kPhi[8] = {-0.999995351f,  -1.15125f,        -0.458468229f,   -0.0539548211f,
-                             0.00850458629f, -0.000929484435f, 6.14394376e-05f, -1.82546e-06f};
-  float a[2 * N], p[2 * N];
+  constexpr float kPhi[11] = {-0.999999881f,    -1.15111041f,    -0.459175467f,   -0.052566696f,
+                              0.00711826188f,   -0.000130872504f, -0.000220343485f, 6.01809223e-05f,
+                              -8.31889884e-06f, 6.23994595e-07f, -2.01010462e-08f};
+  unsigned long long a[N], p[N];
 #pragma unroll
   for (int q = 0; q < N; ++q) {
     const float2 r = f2_split(x[q]);
-    a[2 * q] = fabsf(r.x);
-    a[2 * q + 1] = fabsf(r.y);
+    a[q] = f2(fabsf(r.x), fabsf(r.y));
     x[q] = f2(fmaxf(r.x, 0.f), fmaxf(r.y, 0.f));
   }
 #pragma unroll
-  for (int q = 0; q < 2 * N; ++q) p[q] = fmaf(kPhi[7], a[q], kPhi[6]);
+  for (int q = 0; q < N; ++q) p[q] = f2_fma(f2(kPhi[10], kPhi[10]), a[q], f2(kPhi[9], kPhi[9]));
 #pragma unroll
-  for (int i = 5; i >= 0; --i)
+  for (int i = 8; i >= 0; --i)
 #pragma unroll
-    for (int q = 0; q < 2 * N; ++q) p[q] = fmaf(p[q], a[q], kPhi[i]);
+    for (int q = 0; q < N; ++q) p[q] = f2_fma(p[q], a[q], f2(kPhi[i], kPhi[i]));
 #pragma unroll
   for (int q = 0; q < N; ++q) {
-    const float2 r = f2_split(x[q]);
-    x[q] = f2(fmaf(-a[2 * q], ex2(p[2 * q]), r.x), fmaf(-a[2 * q + 1], ex2(p[2 * q + 1]), r.y));
+    const float2 r = f2_split(x[q]), e = f2_split(p[q]), m = f2_split(a[q]);
+    x[q] = f2(fmaf(-m.x, ex2(e.x), r.x), fmaf(-m.y, ex2(e.y), r.y));
   }
 }
 
@@ -983,8 +988,8 @@ cudaError_t launch_pair_cols(const I8Maps& m, const I8Params& p, bool bf16, bool
 
 // Epilogue warps of the 256-wide tile: eight of 128 columns leave room for a fifth stage; sixteen of 64
 // columns finish a tile sooner, which counts when the GELU takes longer than the tile's MMAs: 8192 x
-// 4096 with GELU, K = 384: 24.8 us with sixteen, 28.4 with eight; K = 768: 30.0 / 29.5; K = 4096: 94.1 /
-// 89.7. Without GELU eight are as fast at K = 384 (50.5 us for 68451 x 1536) and faster above.
+// 4096 with GELU, K = 384: 25.5 us with sixteen, 27.5 with eight; K = 768: 30.1 / 32.8; K = 1024: 34.9 / 36.4;
+// K = 4096: 107.9 / 100.3. Without GELU eight are as fast at K = 384 (50.5 us for 68451 x 1536) and faster above.
 cudaError_t launch_pair_any(const I8Maps& m, const I8Params& p, int bn, bool bf16, bool gelu, bool tma_c, int dev,
                             int sms, cudaStream_t s) {
   if (bn == 128)
@@ -994,8 +999,8 @@ cudaError_t launch_pair_any(const I8Maps& m, const I8Params& p, int bn, bool bf1
     return gelu ? launch_pair_cols<192, 64, true>(m, p, bf16, tma_c, dev, sms, s)
                 : launch_pair_cols<192, 64, false>(m, p, bf16, tma_c, dev, sms, s);
   if (!gelu) return launch_pair_cols<256, 128, false>(m, p, bf16, tma_c, dev, sms, s);
-  return p.K >= 768 ? launch_pair_cols<256, 128, true>(m, p, bf16, tma_c, dev, sms, s)
-                    : launch_pair_cols<256, 64, true>(m, p, bf16, tma_c, dev, sms, s);
+  return p.K >= 1280 ? launch_pair_cols<256, 128, true>(m, p, bf16, tma_c, dev, sms, s)
+                     : launch_pair_cols<256, 64, true>(m, p, bf16, tma_c, dev, sms, s);
 }
 
 template <int BN, bool BF16, bool GELU>
@@ -1078,8 +1083,8 @@ int cluster_room(int log_splits, int sms, int dev) {
 //   pairs: a tile's MMAs take k-blocks (0.024 + 0.00103 bn), its epilogue 0.00613 bn - 0.26 (with GELU 0.0115 bn
 //     - 0.23), the longer of them in every round of tiles but one, in which both count; 2.32 a launch, 0.55 a round.
 // E.g. 64 x 4096 x 4096: bn 64 in 4 parts 5.4 us, bn 32 in 2 parts 5.5, bn 64 whole 6.4; 1024 x 1024 x 4096: bn 64
-// whole 6.8 us, bn 128 in 2 parts 7.7, pairs with bn 256 12.8; pairs, 1024 x 4096 x 1024 with GELU: bn 128 7.4 us,
-// 192 8.8, 256 8.5; 4096 x 4096 x 1024 with GELU: 17.1, 16.7, 18.7; 8192 x 4096 x 4096: 91.6, 90.0, 83.4.
+// whole 6.8 us, bn 128 in 2 parts 7.7, pairs with bn 256 12.8; pairs, 1024 x 4096 x 1024 with GELU: bn 128 7.3 us,
+// 192 8.9, 256 8.3; 4096 x 4096 x 1024 with GELU: 17.8, 17.1, 18.1; 8192 x 4096 x 4096: 91.6, 90.0, 83.4.
 I8Plan choose_plan(int M, int N, int K, bool gelu, int sms, int dev) {
   const int k_blocks = (K + kBK - 1) / kBK;
   I8Plan best{};

@@ -1,0 +1,106 @@
+"""Exactness of the 8-bit linear path on the GPU, finer than one rounding of its 16-bit outputs shows: an output
+is compared with the 64-bit value rounded once, wherever that value lies further from the border between two
+16-bit neighbours than the kernel's 32-bit arithmetic may be off. u = 2^-24 is half a step of fp32."""
+import zlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+DTYPES = [torch.float16, torch.bfloat16]
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def gen(*key):
+    return torch.Generator(device=DEV).manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def gelu_error(z):
+    """(64-bit GELU of z, how far the 32-bit one may be from it), |z| <= 5.75. Of Phi(-a): the fit (1.8e-7 of
+    itself up to a = 4, 2e-6 above), ex2 (2^-22) and the polynomial's fmas in the exponent, each half a step of a
+    partial sum: those partial sums together are under 1 + 3 a + 3 a^2. One rounding of the result follows."""
+    a = z.abs()
+    tail = 0.5 * torch.special.erfc(a / 2**0.5)
+    want = z.clamp(min=0) - a * tail
+    rel = torch.where(a <= 4, 1.8e-7, 2e-6) + 2.0**-22 + 0.6932 * U * (1 + 3 * a + 3 * a * a)
+    return want, a * tail * rel + U * want.abs() * 1.001
+
+
+def decided(want, off, dtype):
+    """Where every value within `off` of `want` has one 16-bit rounding: that of both ends of the interval, since the
+    conversion does not decrease."""
+    lo, hi = (want - off).to(dtype), (want + off).to(dtype)
+    return lo == hi
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [0.5, 1.0, 2.5])
+@pytest.mark.parametrize("kernel", ["pair", "few rows", "one token"])
+def test_gelu_to_32_bits(kernel, size, dtype):
+    """A product of one term: the scale vectors give the GELU's argument to the bit (a_scale or w_scale the value,
+    the others 1)."""
+    import bbh
+
+    count = {"pair": 400_000, "few rows": 60, "one token": 8}[kernel]
+    columns = {"pair": 8, "few rows": 9000, "one token": 70_000}[kernel]
+    g = gen("gelu", kernel, size)
+    a = torch.zeros(count, 16, dtype=torch.int8, device=DEV)
+    w = torch.zeros(columns, 16, dtype=torch.int8, device=DEV)
+    a[:, 0] = 1
+    w[:, 0] = 1
+    wide = kernel != "pair"
+    x = (size * torch.randn(columns if wide else count, generator=g, device=DEV)).clamp(-5.75, 5.75)
+    one = torch.ones(count if wide else columns, device=DEV)
+    c = bbh.linear_i8(a, one, w, x, gelu=True, dtype=dtype) if wide else bbh.linear_i8(a, x, w, one, gelu=True, dtype=dtype)
+    c = c if wide else c.t()
+    assert torch.equal(c, c[:1].expand_as(c))
+    want, off = gelu_error(x.double())
+    sure = decided(want, off, dtype)
+    assert sure.double().mean().item() > 0.99
+    assert torch.equal(c[0][sure], want.to(dtype)[sure])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,D,F", [(1, 384, 1536), (50, 384, 1536), (1024, 1024, 4096), (1000, 333, 1001)])
+def test_ffn_block_stage_by_stage(M, D, F, dtype):
+    """norm -> up + GELU -> quantise -> down, each stage in 64 bits from what the stage in front returned: a 16-bit
+    output is the 64-bit value's rounding wherever 32-bit arithmetic leaves no doubt, and the integers of the GELU's
+    output are those of the 64-bit quotient, all of them."""
+    import bbh
+
+    g = gen("stages", M, D, F)
+    rand = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    x, r = rand(M, D).to(dtype), rand(M, D).to(dtype)
+    nw = (1 + 0.1 * rand(D)).to(dtype)
+    up, up_s = bbh.quantize_i8((rand(F, D) / D**0.5).to(dtype))
+    down, down_s = bbh.quantize_i8((rand(D, F) / F**0.5).to(dtype))
+    bu, bd = (0.1 * rand(F)).to(dtype), (0.1 * rand(D)).to(dtype)
+    q, s, v = bbh.rmsnorm_i8(x, nw, residual=r)
+    h = bbh.linear_i8(q, s, up, up_s, bu, gelu=True, dtype=dtype)
+    q2, s2 = bbh.quantize_i8(h)
+    y = bbh.linear_i8(q2, s2, down, down_s, bd, dtype=dtype)
+    product = lambda a, sa, w, sw: (a.double() @ w.double().T) * sa.double()[:, None] * sw.double()
+    p = product(q, s, up, up_s)
+    z = p + bu.double()
+    # int -> fp32, * a_scale, * w_scale + bias: three roundings, the first two of the product alone; GELU's slope is
+    # under 1.13
+    want, off = gelu_error(z)
+    off = off + 1.13 * U * (2 * p.abs() + z.abs()) * 1.001
+    sure = decided(want, off, dtype) & (z.abs() <= 5.75)
+    assert sure.double().mean().item() > 0.99
+    assert torch.equal(h[sure], want.to(dtype)[sure])
+    t = h.double()
+    assert torch.equal(q2.double(), torch.round(t * 127 / t.abs().amax(1, keepdim=True)))
+    p = product(q2, s2, down, down_s)
+    want = p + bd.double()
+    sure = decided(want, U * (2 * p.abs() + want.abs()) * 1.001, dtype)
+    assert sure.double().mean().item() > 0.99
+    assert torch.equal(y[sure], want.to(dtype)[sure])
