@@ -115,17 +115,25 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// min(|x|, 16) that keeps a NaN (fminf drops it)
+__device__ __forceinline__ float abs_to_16(float x) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(x)), "f"(16.f));
+  return d;
+}
+
 // erf-GELU, x Phi(x) = max(x, 0) - |x| Phi(-|x|), of N pairs of fp32 values side by side (which hides
 // the fmas' latency). log2 Phi(-a) is close to a parabola and is evaluated as a polynomial of degree 10
 // in a (this project's own least-squares fit on [0, 5.75], weighted by what an error means to the
 // output and reweighted to equal ripple): Phi(-a) is within 1.8e-7 of itself up to a = 4, 2e-6 up to 5.75;
-// beyond, the polynomial keeps falling, and Phi with it, so no clamp is needed. With the roundings of the
-// sum and of ex2 the output is within 1e-7 max(|x|, 1).
+// beyond, the polynomial keeps falling until ex2 gives 0 (from a = 11.5 on); a ends at 16, because infinity times that
+// 0 would be NaN: +inf stays +inf, -inf gives 0, and only NaN gives NaN. With the roundings of the sum and of ex2
+// the output is within 1e-7 max(|x|, 1).
 // Why this degree: of normal x 0.009 % of the fp16 outputs are the other neighbour of the exact value, 0.018 %
 // with fp32's erf. Degree 7 (Phi within 5.8e-6) has 0.20 %, and a quantiser behind the layer then rounds ten times
 // as many of its integers the other way, each of which the next layer spreads over a row; degree 9 0.018 to
 // 0.03 %. 68451 x 1536 x 384: 68.9 us with degree 7 one value at a time, here, in packed pairs (half the
-// issue slots), 73.8; degree 9 71.8; degree 10 one value at a time 82.3.
+// issue slots), 74.3; degree 9 72.9; degree 10 one value at a time 82.3.
 template <int N>
 __device__ __forceinline__ void gelu2(unsigned long long (&x)[N]) {
   constexpr float kPhi[11] = {-0.999999881f,    -1.15111041f,    -0.459175467f,   -0.052566696f,
@@ -135,7 +143,7 @@ __device__ __forceinline__ void gelu2(unsigned long long (&x)[N]) {
 #pragma unroll
   for (int q = 0; q < N; ++q) {
     const float2 r = f2_split(x[q]);
-    a[q] = f2(fabsf(r.x), fabsf(r.y));
+    a[q] = f2(abs_to_16(r.x), abs_to_16(r.y));
     x[q] = f2(fmaxf(r.x, 0.f), fmaxf(r.y, 0.f));
   }
 #pragma unroll

@@ -104,3 +104,30 @@ def test_ffn_block_stage_by_stage(M, D, F, dtype):
     sure = decided(want, U * (2 * p.abs() + want.abs()) * 1.001, dtype)
     assert sure.double().mean().item() > 0.99
     assert torch.equal(y[sure], want.to(dtype)[sure])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N", [(1, 64), (3, 70_000), (40, 64), (300, 1000), (3000, 1001), (5000, 4096)])
+def test_gelu_of_infinities(M, N, dtype):
+    """x Phi(x) is +inf at +inf and 0 at -inf; NaN only of NaN. An infinite bias, an infinite scale, and finite values
+    far out, each in columns of its own next to ordinary ones."""
+    import bbh
+
+    inf, nan = float("inf"), float("nan")
+    g = gen("infinities", M, N)
+    a = torch.randint(1, 100, (M, 16), generator=g, device=DEV, dtype=torch.int8)
+    w = torch.randint(1, 100, (N, 16), generator=g, device=DEV, dtype=torch.int8)
+    sa = torch.full((M,), 1e-3, device=DEV)
+    sw = torch.full((N,), 1e-3, device=DEV)
+    b = torch.zeros(N, dtype=dtype, device=DEV)
+    plain = bbh.linear_i8(a, sa, w, sw, b, gelu=True, dtype=dtype)
+    big = 6e4 if dtype is torch.float16 else 3e38
+    b[1::9], b[3::9], b[5::9], b[7::9] = inf, -inf, nan, big
+    sw[2::9], sw[6::9] = inf, -inf
+    sw[8::9] = -3e38
+    c = bbh.linear_i8(a, sa, w, sw, b, gelu=True, dtype=dtype)
+    assert bool((c[:, 1::9] == inf).all()) and bool((c[:, 2::9] == inf).all())
+    assert bool((c[:, 3::9] == 0).all()) and bool((c[:, 6::9] == 0).all()) and bool((c[:, 8::9] == 0).all())
+    assert bool(torch.isnan(c[:, 5::9]).all())
+    assert bool((c[:, 7::9] >= big * 0.99).all()) and not bool(torch.isnan(c[:, 7::9]).any())
+    assert torch.equal(c[:, 0::9], plain[:, 0::9]) and torch.equal(c[:, 4::9], plain[:, 4::9])
