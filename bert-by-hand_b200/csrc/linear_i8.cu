@@ -10,6 +10,9 @@
 //    its columns, K split over the CTAs of a cluster, partial sums added in shared memory
 //    (int32: exact in any order); both fed by 128-byte-swizzled TMA tiles of 128 int8 along K;
 //  * linear_i8_few_kernel -- one to 16 tokens: the weights straight from memory into registers.
+// A launch starts while the one in front still runs (griddepcontrol), and that one may write any operand: global
+// memory is read after pdl_wait() only, and never through the non-coherent path (__ldg, const __restrict__),
+// which is for what stays constant as long as the kernel lives.
 // Every wait is bounded (mbar_wait); one that runs out sets the device error word and the
 // kernel returns.
 #include "common.cuh"
@@ -426,12 +429,12 @@ __global__ void __launch_bounds__(I8PairCfg<BN, COLS>::THREADS, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = tile_m0(t) + quad * 32 + row_t + 8 * i;
-        sa_next[i] = row < p.M ? __ldg(p.a_scale + row) : 0.f;
+        sa_next[i] = row < p.M ? p.a_scale[row] : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < COLS / 32; ++i) {
         const int c = tile_n0(t) + part * COLS + 32 * i + lane;
-        sw_next[i] = c < p.N ? __ldg(p.w_scale + c) : 0.f;
+        sw_next[i] = c < p.N ? p.w_scale[c] : 0.f;
         b_next[i] = p.bias && c < p.N ? bias_f32<BF16>(p.bias + c) : 0.f;
       }
     };
@@ -590,7 +593,7 @@ struct I8SmallCfg {
 template <int BN, bool BF16, bool GELU>
 __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
     linear_i8_small_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                           const I8Params p, const int log_splits, const int8_t* __restrict__ W, const int64_t ldw) {
+                           const I8Params p, const int log_splits, const int8_t* W, const int64_t ldw) {
   using Cfg = I8SmallCfg<BN>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -723,9 +726,9 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
   bool ok = true;
   if (epi) {
     const int e = threadIdx.x - 64;
-    if (e < BN) s_sa[e] = e < tokens ? __ldg(p.a_scale + m0 + e) : 0.f;
+    if (e < BN) s_sa[e] = e < tokens ? p.a_scale[m0 + e] : 0.f;
     if (n < p.N) {
-      const float s = __ldg(p.w_scale + n);
+      const float s = p.w_scale[n];
       const float b = p.bias ? bias_f32<BF16>(p.bias + n) : 0.f;
       sw = f2(s, s);
       bias = f2(b, b);
@@ -846,7 +849,7 @@ __device__ __forceinline__ void mma_i8(int (&c)[4], uint32_t a0, uint32_t a1, ui
 
 // 16 bytes of an int8 row from k on, zeros behind its end (and nothing read there).
 __device__ __forceinline__ uint4 load_k16(const int8_t* row, int k, int K) {
-  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
   const int r = k < K ? K - k : 0;  // 0 .. 15 bytes: an 8-, a 4-, a 2- and a 1-byte load
   const int8_t* at = row + k;
   uint64_t lo = 0, rest = 0;
@@ -866,7 +869,7 @@ __device__ __forceinline__ uint4 load_k16(const int8_t* row, int k, int K) {
 // MT: token tiles of 8. U: 64-byte steps in flight per warp.
 template <int MT, int U, bool BF16, bool GELU>
 __global__ void __launch_bounds__(32 * kFewWarps)
-    linear_i8_few_kernel(const int8_t* __restrict__ A, const int64_t lda, const int8_t* __restrict__ W,
+    linear_i8_few_kernel(const int8_t* A, const int64_t lda, const int8_t* W,
                          const int64_t ldw, const I8Params p) {
   __shared__ int part[kFewWarps][MT * 128];
   pdl_launch_dependents();
@@ -918,9 +921,9 @@ __global__ void __launch_bounds__(32 * kFewWarps)
   }
   const int64_t n = n0 + c;
   const bool one = n < p.N, two = n + 1 < p.N;
-  const float sa = __ldg(p.a_scale + tok);
+  const float sa = p.a_scale[tok];
   const float b0 = p.bias && one ? bias_f32<BF16>(p.bias + n) : 0.f, b1 = p.bias && two ? bias_f32<BF16>(p.bias + n + 1) : 0.f;
-  unsigned long long y[1] = {dequant2(s0, s1, f2(sa, sa), f2(one ? __ldg(p.w_scale + n) : 0.f, two ? __ldg(p.w_scale + n + 1) : 0.f),
+  unsigned long long y[1] = {dequant2(s0, s1, f2(sa, sa), f2(one ? p.w_scale[n] : 0.f, two ? p.w_scale[n + 1] : 0.f),
                                       f2(b0, b1))};
   uint32_t o[1];
   finish2<BF16, GELU>(y, o);
