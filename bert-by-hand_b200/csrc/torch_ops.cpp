@@ -5,13 +5,15 @@
 //
 // Arguments are positional (bbh.py has the signatures and the documentation). TypeError and
 // ValueError say what is wrong with a tensor, BBHError (given by bbh.py) what the C ABI
-// refused. No gradient is recorded.
+// refused; errors of torch's own are torch's (torch.OutOfMemoryError where an output cannot be
+// allocated). No gradient is recorded.
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
@@ -53,8 +55,10 @@ PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F f) {
       PyErr_SetObject(g_bbh_error, o);
       Py_DECREF(o);
     }
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception&) {
+    torch::translate_exception_to_python(std::current_exception());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
   }
   return nullptr;
 }
