@@ -42,6 +42,17 @@ void check(int rc) {
   if (rc != BBH_OK) throw Failed(rc);
 }
 
+// The interpreter is free while this lives: an allocation may wait for the device and a launch for room in the
+// queue, and what they wait for (a host function of a stream in front, another thread) may need the interpreter.
+// Between the reading of the arguments and the wrapping of results; a throw takes the lock back first.
+struct NoGil {
+  PyThreadState* state = PyEval_SaveThread();
+  NoGil() = default;
+  NoGil(const NoGil&) = delete;
+  NoGil& operator=(const NoGil&) = delete;
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
+
 // Runs f, turning its exceptions into Python's.
 template <typename F>
 PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F f) {
@@ -195,15 +206,18 @@ PyObject* rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (eps == -1.0 && PyErr_Occurred()) return nullptr;
     Rows yr;
     if (a[4] != Py_None) yr = rows(given(a[4], "out"), k.dev, k.type, k.m, k.d, "out");
-    const c10::cuda::CUDAGuard on(k.dev);
-    k.make_sum(a[5]);
     at::Tensor y;
-    if (a[4] == Py_None) {
-      y = make({k.m, k.d}, k.type, k.dev);
-      yr = {y.data_ptr(), k.d};
+    {
+      const NoGil no_gil;
+      const c10::cuda::CUDAGuard on(k.dev);
+      k.make_sum(a[5]);
+      if (a[4] == Py_None) {
+        y = make({k.m, k.d}, k.type, k.dev);
+        yr = {y.data_ptr(), k.d};
+      }
+      check(bbh_rmsnorm(ptr<U16>(k.xr), k.xr.ld, ptr<U16>(k.rr), k.rr.ld, k.weight, ptr<U16>(yr), yr.ld, ptr<U16>(k.sr),
+                        k.sr.ld, as_int(k.m), as_int(k.d), static_cast<float>(eps), k.code, stream_of(k.dev)));
     }
-    check(bbh_rmsnorm(ptr<U16>(k.xr), k.xr.ld, ptr<U16>(k.rr), k.rr.ld, k.weight, ptr<U16>(yr), yr.ld, ptr<U16>(k.sr),
-                      k.sr.ld, as_int(k.m), as_int(k.d), static_cast<float>(eps), k.code, stream_of(k.dev)));
     PyObject* oy = result(a[4], y);
     return k.residual ? tuple({oy, result(a[5], k.sum)}) : oy;
   });
@@ -215,12 +229,17 @@ PyObject* rmsnorm_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     NormArgs k(a[0], a[1], a[3], a[4]);
     const double eps = PyFloat_AsDouble(a[2]);
     if (eps == -1.0 && PyErr_Occurred()) return nullptr;
-    const c10::cuda::CUDAGuard on(k.dev);
-    k.make_sum(a[4]);
-    const at::Tensor q = make_i8(k.m, k.d, k.dev), scale = make({k.m}, at::kFloat, k.dev);
-    check(bbh_rmsnorm_i8(ptr<U16>(k.xr), k.xr.ld, ptr<U16>(k.rr), k.rr.ld, k.weight, static_cast<int8_t*>(q.data_ptr()),
-                         q.stride(0), static_cast<float*>(scale.data_ptr()), ptr<U16>(k.sr), k.sr.ld, as_int(k.m),
-                         as_int(k.d), static_cast<float>(eps), k.code, stream_of(k.dev)));
+    at::Tensor q, scale;
+    {
+      const NoGil no_gil;
+      const c10::cuda::CUDAGuard on(k.dev);
+      k.make_sum(a[4]);
+      q = make_i8(k.m, k.d, k.dev);
+      scale = make({k.m}, at::kFloat, k.dev);
+      check(bbh_rmsnorm_i8(ptr<U16>(k.xr), k.xr.ld, ptr<U16>(k.rr), k.rr.ld, k.weight, static_cast<int8_t*>(q.data_ptr()),
+                           q.stride(0), static_cast<float*>(scale.data_ptr()), ptr<U16>(k.sr), k.sr.ld, as_int(k.m),
+                           as_int(k.d), static_cast<float>(eps), k.code, stream_of(k.dev)));
+    }
     PyObject *oq = THPVariable_Wrap(q), *os = THPVariable_Wrap(scale);
     return k.residual ? tuple({oq, os, result(a[4], k.sum)}) : tuple({oq, os});
   });
@@ -235,10 +254,15 @@ PyObject* quantize_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int code = dtype_code(x.scalar_type());
     const int64_t m = x.size(0), d = x.size(1);
     const Rows xr = rows(x, dev, x.scalar_type(), m, d, "x");
-    const c10::cuda::CUDAGuard on(dev);
-    const at::Tensor q = make_i8(m, d, dev), scale = make({m}, at::kFloat, dev);
-    check(bbh_quantize_i8(ptr<U16>(xr), xr.ld, static_cast<int8_t*>(q.data_ptr()), q.stride(0),
-                          static_cast<float*>(scale.data_ptr()), as_int(m), as_int(d), code, stream_of(dev)));
+    at::Tensor q, scale;
+    {
+      const NoGil no_gil;
+      const c10::cuda::CUDAGuard on(dev);
+      q = make_i8(m, d, dev);
+      scale = make({m}, at::kFloat, dev);
+      check(bbh_quantize_i8(ptr<U16>(xr), xr.ld, static_cast<int8_t*>(q.data_ptr()), q.stride(0),
+                            static_cast<float*>(scale.data_ptr()), as_int(m), as_int(d), code, stream_of(dev)));
+    }
     return tuple({THPVariable_Wrap(q), THPVariable_Wrap(scale)});
   });
 }
@@ -257,14 +281,17 @@ PyObject* dequantize_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     float* scale = vec<float>(&given(a[1], "scale"), dev, at::kFloat, m, "scale");
     Rows yr;
     if (out) yr = rows(*out, dev, type, m, d, "out");
-    const c10::cuda::CUDAGuard on(dev);
     at::Tensor y;
-    if (!out) {
-      y = make({m, d}, type, dev);
-      yr = {y.data_ptr(), d};
+    {
+      const NoGil no_gil;
+      const c10::cuda::CUDAGuard on(dev);
+      if (!out) {
+        y = make({m, d}, type, dev);
+        yr = {y.data_ptr(), d};
+      }
+      check(bbh_dequantize_i8(ptr<int8_t>(qr), qr.ld, scale, ptr<U16>(yr), yr.ld, as_int(m), as_int(d), code,
+                              stream_of(dev)));
     }
-    check(bbh_dequantize_i8(ptr<int8_t>(qr), qr.ld, scale, ptr<U16>(yr), yr.ld, as_int(m), as_int(d), code,
-                            stream_of(dev)));
     return result(a[3], y);
   });
 }
@@ -288,14 +315,17 @@ PyObject* linear_i8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (gelu < 0) return nullptr;
     Rows cr;
     if (out) cr = rows(*out, dev, type, M, N, "out");
-    const c10::cuda::CUDAGuard on(dev);
     at::Tensor C;
-    if (!out) {
-      C = make({M, N}, type, dev);
-      cr = {C.data_ptr(), N};
+    {
+      const NoGil no_gil;
+      const c10::cuda::CUDAGuard on(dev);
+      if (!out) {
+        C = make({M, N}, type, dev);
+        cr = {C.data_ptr(), N};
+      }
+      check(bbh_linear_i8(ptr<int8_t>(ar), ar.ld, sa, ptr<int8_t>(wr), wr.ld, sw, bias, ptr<U16>(cr), cr.ld, as_int(M),
+                          as_int(N), as_int(K), gelu, code, stream_of(dev)));
     }
-    check(bbh_linear_i8(ptr<int8_t>(ar), ar.ld, sa, ptr<int8_t>(wr), wr.ld, sw, bias, ptr<U16>(cr), cr.ld, as_int(M),
-                        as_int(N), as_int(K), gelu, code, stream_of(dev)));
     return result(a[7], C);
   });
 }

@@ -1,4 +1,7 @@
-"""What the Python calls of the 8-bit linear path do besides launching: errors."""
+"""What the Python calls of the 8-bit linear path do besides launching: errors, other threads."""
+import threading
+import time
+
 import pytest
 import torch
 
@@ -23,3 +26,44 @@ def test_out_of_memory_is_torchs_error():
     with pytest.raises(torch.OutOfMemoryError, match="out of memory"):
         bbh.linear_i8(q, s, q, s)
     assert bool((bbh.linear_i8(q[:5], s[:5], q[:7], s[:7]) == 0).all())
+
+
+@pytest.mark.parametrize("name", ["rmsnorm", "rmsnorm_i8", "quantize_i8", "dequantize_i8", "linear_i8"])
+def test_other_threads_run_while_a_launch_waits(name):
+    """A stream takes about a thousand launches; one more waits for room. 1,500 calls behind a second of work on the
+    device: the thread that makes them waits most of that second in a launch, another one goes on all the time."""
+    import bbh
+
+    x = torch.ones(2, 64, dtype=torch.float16, device=DEV)
+    q, s = bbh.quantize_i8(x)
+    out, wide = torch.empty_like(x), torch.empty(2, 2, dtype=torch.float16, device=DEV)
+    call = {"rmsnorm": lambda: bbh.rmsnorm(x, out=out), "rmsnorm_i8": lambda: bbh.rmsnorm_i8(x),
+            "quantize_i8": lambda: bbh.quantize_i8(x), "dequantize_i8": lambda: bbh.dequantize_i8(q, s, out=out),
+            "linear_i8": lambda: bbh.linear_i8(q, s, q, s, out=wide)}[name]
+    call()
+    torch.cuda.synchronize()
+    times, stop = [], threading.Event()
+
+    def tick():
+        while not stop.wait(0.002):
+            times.append(time.perf_counter())
+
+    t = threading.Thread(target=tick)
+    t.start()
+    try:
+        began = time.perf_counter()
+        torch.cuda._sleep(2_000_000_000)
+        longest = 0.0
+        for _ in range(1500):
+            a = time.perf_counter()
+            call()
+            longest = max(longest, time.perf_counter() - a)
+        torch.cuda.synchronize()
+        ended = time.perf_counter()
+    finally:
+        stop.set()
+        t.join()
+    inside = [began, *(v for v in times if began < v < ended), ended]
+    gap = max(b - a for a, b in zip(inside, inside[1:]))
+    assert longest > 0.5, "no launch had to wait"
+    assert gap < 0.4 * longest, (gap, longest)
