@@ -236,11 +236,14 @@ __device__ __forceinline__ uint2 low_bytes(const uint32_t* b) {
 }
 
 // 127 / top from the hardware's reciprocal (off by 2^-23 at most) and 3 * 2^-23 more, so that with its two
-// roundings it is above 127 / top by 0 to 5 * 2^-23 of it.
+// roundings it is above 127 / top by 0 to 5 * 2^-23 of it. Above 2^126 (bf16) the reciprocal would be subnormal, with
+// steps of up to 2^-21 of itself: such a top is divided by 16 first, and the quotient at the end.
+template <bool BF16>
 __device__ __forceinline__ float steps_per_unit(float top) {
+  const float unit = BF16 && top > 0x1p125f ? 0x1p-4f : 1.f;
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
-  return r * 127.f * (1.f + 3 * 0x1p-23f);
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top * unit));
+  return r * 127.f * (1.f + 3 * 0x1p-23f) * unit;
 }
 
 // 127 / top to half an ulp and a little: one Newton step, for values that do not meet exact halves (kRowNormI8).
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(kRowMaxBlock, V <= 4 && CUT != kSingle ? 2 : 1
     // that whatever is computed from it is NaN too.
     const bool finite = top <= FLT_MAX;
     const bool zero = !finite || top < 0x1p-120f;
-    const float inv = MODE == kRowQuant ? steps_per_unit(zero ? 1.f : top) : steps_per_unit_near(zero ? 1.f : top);
+    const float inv = MODE == kRowQuant ? steps_per_unit<BF16>(zero ? 1.f : top) : steps_per_unit_near(zero ? 1.f : top);
     bool ties = false;
     float rest = 0.f;
     if constexpr (MODE == kRowQuant) {

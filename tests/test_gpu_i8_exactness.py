@@ -131,3 +131,21 @@ def test_gelu_of_infinities(M, N, dtype):
     assert bool(torch.isnan(c[:, 5::9]).all())
     assert bool((c[:, 7::9] >= big * 0.99).all()) and not bool(torch.isnan(c[:, 7::9]).any())
     assert torch.equal(c[:, 0::9], plain[:, 0::9]) and torch.equal(c[:, 4::9], plain[:, 4::9])
+
+
+def test_half_to_even_in_rows_near_the_end_of_bf16():
+    """Every bf16 value in [2^120, 2^128) as a row's maximum, its half (63.5 steps, to 64) and its small parts: near the
+    upper end a reciprocal of the maximum is no normal fp32 number."""
+    import bbh
+
+    bits = torch.arange(0x7B80, 0x7F80, device=DEV, dtype=torch.int32).to(torch.int16)
+    top = bits.view(torch.bfloat16)
+    assert top[0].item() == 2.0**120 and top[-1].item() == torch.finfo(torch.bfloat16).max
+    x = torch.randn(top.numel(), 64, generator=gen("bf16 end"), device=DEV).clamp(-1, 1).bfloat16() * top[:, None]
+    x[:, 0], x[:, 1], x[:, 2], x[:, 3] = top, top / 2, -top / 2, -top
+    for k in range(4, 12):
+        x[:, k] = top * 2.0 ** (2 - k)
+    q, s = bbh.quantize_i8(x)
+    want = torch.round(x.double() * 127 / top.double()[:, None])
+    assert torch.equal(q.double(), want)
+    assert bool(((s.double() * 127 / top.double() - 1).abs() <= U).all())
