@@ -81,6 +81,7 @@ _SIGS = {
     "bbh_quantize_i8": (_I, [_P, _L, _P, _L, _P, _I, _I, _I, _P]),
     "bbh_dequantize_i8": (_I, [_P, _L, _P, _P, _L, _I, _I, _I, _P]),
     "bbh_linear_i8": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _P]),
+    "bbh_linear_i8_plan": (_I, [_I, _I, _I, _I, ctypes.POINTER(_I)]),
     "bbh_linear_i8_device_error": (_I, [_I]),
     "bbh_embed_varlen_static": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P]),
     "bbh_static_device_error": (_I, []),
@@ -613,6 +614,14 @@ def linear_i8(A, a_scale, W, w_scale, bias=None, gelu=False, dtype=torch.float16
         with _on(A, stream):
             return linear_i8(A, a_scale, W, w_scale, bias, gelu, dtype, out)
     return (_ops_module or _ops()).linear_i8(A, a_scale, W, w_scale, bias, gelu, dtype, out)
+
+
+def linear_i8_plan(M: int, N: int, K: int, gelu: bool = False):
+    """The kernel that linear_i8 runs for these sizes on the current device: ("few", tiles of 8 tokens, steps of K in
+    flight), ("split", tokens a tile, CTAs that share K) or ("pair", columns a tile, columns an epilogue warp)."""
+    plan = (ctypes.c_int * 3)()
+    _check(lib().bbh_linear_i8_plan(M, N, K, 1 if gelu else 0, plan))
+    return ("few", "split", "pair")[plan[0]], plan[1], plan[2]
 
 
 def linear_i8_device_error(reset: bool = True) -> int:

@@ -997,12 +997,14 @@ cudaError_t launch_pair_cols(const I8Maps& m, const I8Params& p, bool bf16, bool
                : launch_pair_i8<BN, COLS, false, GELU, false>(m, p, dev, sms, s);
 }
 
-// Epilogue warps of the 256-wide tile: eight of 128 columns leave room for a fifth stage; sixteen of 64
-// columns finish a tile sooner, which counts when the GELU takes longer than the tile's MMAs: 8192 x
+// Columns of an epilogue warp. For the 256-wide tile, eight warps of 128 columns leave room for a fifth stage;
+// sixteen of 64 columns finish a tile sooner, which counts when the GELU takes longer than the tile's MMAs: 8192 x
 // 4096 with GELU, K = 384: 25.5 us with sixteen, 27.5 with eight; K = 768: 30.1 / 32.8; K = 1024: 34.9 / 36.4;
 // K = 4096: 107.9 / 100.3. Without GELU eight are as fast at K = 384 (50.5 us for 68451 x 1536) and faster above.
-cudaError_t launch_pair_any(const I8Maps& m, const I8Params& p, int bn, bool bf16, bool gelu, bool tma_c, int dev,
-                            int sms, cudaStream_t s) {
+int pair_cols(int bn, int K, bool gelu) { return bn < 256 || (gelu && K < 1280) ? 64 : 128; }
+
+cudaError_t launch_pair_any(const I8Maps& m, const I8Params& p, int bn, int cols, bool bf16, bool gelu, bool tma_c,
+                            int dev, int sms, cudaStream_t s) {
   if (bn == 128)
     return gelu ? launch_pair_cols<128, 64, true>(m, p, bf16, tma_c, dev, sms, s)
                 : launch_pair_cols<128, 64, false>(m, p, bf16, tma_c, dev, sms, s);
@@ -1010,30 +1012,32 @@ cudaError_t launch_pair_any(const I8Maps& m, const I8Params& p, int bn, bool bf1
     return gelu ? launch_pair_cols<192, 64, true>(m, p, bf16, tma_c, dev, sms, s)
                 : launch_pair_cols<192, 64, false>(m, p, bf16, tma_c, dev, sms, s);
   if (!gelu) return launch_pair_cols<256, 128, false>(m, p, bf16, tma_c, dev, sms, s);
-  return p.K >= 1280 ? launch_pair_cols<256, 128, true>(m, p, bf16, tma_c, dev, sms, s)
+  return cols == 128 ? launch_pair_cols<256, 128, true>(m, p, bf16, tma_c, dev, sms, s)
                      : launch_pair_cols<256, 64, true>(m, p, bf16, tma_c, dev, sms, s);
 }
 
 template <int BN, bool BF16, bool GELU>
-cudaError_t launch_small_i8(const I8Maps& m, const I8Params& p, int log_splits, int dev, cudaStream_t s) {
+cudaError_t launch_small_i8(const I8Maps& m, const I8Params& p, int splits, int dev, cudaStream_t s) {
   using Cfg = I8SmallCfg<BN>;
   static bool done[64] = {};
   auto kern = linear_i8_small_kernel<BN, BF16, GELU>;
   const cudaError_t e = opt_in(kern, Cfg::SMEM, done, dev);
   if (e != cudaSuccess) return e;
+  int log_splits = 0;
+  while ((1 << log_splits) < splits) ++log_splits;
   const dim3 grid(static_cast<unsigned>(((p.N - 1) / 128 + 1) << log_splits), static_cast<unsigned>((p.M - 1) / BN + 1));
-  return launch_ex(kern, grid, dim3(Cfg::THREADS), Cfg::SMEM, s, true, 1 << log_splits, m.W, m.A, p, log_splits,
+  return launch_ex(kern, grid, dim3(Cfg::THREADS), Cfg::SMEM, s, true, splits, m.W, m.A, p, log_splits,
                    m.w, m.ldw);
 }
 
 template <int BN>
-cudaError_t launch_small_bn(const I8Maps& m, const I8Params& p, bool bf16, bool gelu, int log_splits, int dev,
+cudaError_t launch_small_bn(const I8Maps& m, const I8Params& p, bool bf16, bool gelu, int splits, int dev,
                             cudaStream_t s) {
   if (bf16)
-    return gelu ? launch_small_i8<BN, true, true>(m, p, log_splits, dev, s)
-                : launch_small_i8<BN, true, false>(m, p, log_splits, dev, s);
-  return gelu ? launch_small_i8<BN, false, true>(m, p, log_splits, dev, s)
-              : launch_small_i8<BN, false, false>(m, p, log_splits, dev, s);
+    return gelu ? launch_small_i8<BN, true, true>(m, p, splits, dev, s)
+                : launch_small_i8<BN, true, false>(m, p, splits, dev, s);
+  return gelu ? launch_small_i8<BN, false, true>(m, p, splits, dev, s)
+              : launch_small_i8<BN, false, false>(m, p, splits, dev, s);
 }
 
 template <int MT, int U>
@@ -1045,15 +1049,20 @@ cudaError_t launch_few(const int8_t* A, int64_t lda, const int8_t* W, int64_t ld
   return gelu ? go(linear_i8_few_kernel<MT, U, false, true>) : go(linear_i8_few_kernel<MT, U, false, false>);
 }
 
-// Steps in flight: as many as a warp has (512 bytes of K each), where the CTAs are too few to keep memory
-// busy otherwise. 1 x 4096 x 4096: 8 steps 3.3 us, 4 steps 4.0, 2 steps 4.7; 1 x 384 x 384: 2.5, 1.9, 1.5;
-// 1 x 16384 x 4096 (1,024 CTAs): 10.3, 9.8, 9.2.
-cudaError_t launch_few_any(const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, const I8Params& p, bool bf16,
-                           bool gelu, int sms, cudaStream_t s) {
-  if (p.M > 8) return launch_few<2, 2>(A, lda, W, ldw, p, bf16, gelu, s);
-  if (p.K <= 1024 || p.N > 32 * sms) return launch_few<1, 2>(A, lda, W, ldw, p, bf16, gelu, s);
-  return p.K <= 2048 ? launch_few<1, 4>(A, lda, W, ldw, p, bf16, gelu, s)
-                     : launch_few<1, 8>(A, lda, W, ldw, p, bf16, gelu, s);
+// Steps in flight of the kernel for one to 16 tokens: as many as a warp has (512 bytes of K each), where the CTAs are
+// too few to keep memory busy otherwise. 1 x 4096 x 4096: 8 steps 3.3 us, 4 steps 4.0, 2 steps 4.7; 1 x 384 x
+// 384: 2.5, 1.9, 1.5; 1 x 16384 x 4096 (1,024 CTAs): 10.3, 9.8, 9.2.
+int few_steps(int M, int N, int K, int sms) {
+  if (M > 8 || K <= 1024 || N > 32 * sms) return 2;
+  return K <= 2048 ? 4 : 8;
+}
+
+cudaError_t launch_few_any(const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, const I8Params& p, int tiles,
+                           int steps, bool bf16, bool gelu, cudaStream_t s) {
+  if (tiles == 2) return launch_few<2, 2>(A, lda, W, ldw, p, bf16, gelu, s);
+  if (steps == 2) return launch_few<1, 2>(A, lda, W, ldw, p, bf16, gelu, s);
+  return steps == 4 ? launch_few<1, 4>(A, lda, W, ldw, p, bf16, gelu, s)
+                    : launch_few<1, 8>(A, lda, W, ldw, p, bf16, gelu, s);
 }
 
 // Whether that kernel takes less time than the tcgen05 one (us, few rows / tcgen05), with the weights in L2: 1 x 4096
@@ -1066,10 +1075,11 @@ bool few_is_faster(int M, int N, int K, int sms) {
   return M <= 16 && K <= 2048 && weights <= (int64_t(4) << 20);
 }
 
+// Which kernel a call runs: BBH_I8_FEW with `tile` 8-token tiles and `part` steps in flight, BBH_I8_SPLIT with `tile`
+// tokens a tile and K in `part` (a power of two) CTAs, BBH_I8_PAIR with `tile` columns a tile and `part` a warp of
+// the epilogue.
 struct I8Plan {
-  bool pair;
-  int bn;          // column tile of the pair kernel, token tile of the other
-  int log_splits;  // K split over 2^log_splits CTAs
+  int kernel, tile, part;
 };
 
 // CTAs of the few-rows kernel that run at once in clusters of 2^log_splits, in clusters (all token tiles
@@ -1097,6 +1107,7 @@ int cluster_room(int log_splits, int sms, int dev) {
 // whole 6.8 us, bn 128 in 2 parts 7.7, pairs with bn 256 12.8; pairs, 1024 x 4096 x 1024 with GELU: bn 128 7.3 us,
 // 192 8.9, 256 8.3; 4096 x 4096 x 1024 with GELU: 17.8, 17.1, 18.1; 8192 x 4096 x 4096: 91.6, 90.0, 83.4.
 I8Plan choose_plan(int M, int N, int K, bool gelu, int sms, int dev) {
+  if (few_is_faster(M, N, K, sms)) return {BBH_I8_FEW, M > 8 ? 2 : 1, few_steps(M, N, K, sms)};
   const int k_blocks = (K + kBK - 1) / kBK;
   I8Plan best{};
   double best_us = DBL_MAX;
@@ -1109,7 +1120,7 @@ I8Plan choose_plan(int M, int N, int K, bool gelu, int sms, int dev) {
     const int64_t tiles = (int64_t(M) + 255) / 256 * ((N - 1) / bn + 1);
     const double rounds = static_cast<double>((tiles - 1) / (sms / 2) + 1);
     const double mma = k_blocks * (0.024 + 0.00103 * bn), epi = gelu ? 0.0115 * bn - 0.23 : 0.00613 * bn - 0.26;
-    consider(2.32 + mma + epi + (rounds - 1) * (mma > epi ? mma : epi) + 0.55 * rounds, {true, bn, 0});
+    consider(2.32 + mma + epi + (rounds - 1) * (mma > epi ? mma : epi) + 0.55 * rounds, {BBH_I8_PAIR, bn, pair_cols(bn, K, gelu)});
   }
   const int64_t ch_tiles = (N - 1) / 128 + 1;
   for (int bn = 16; bn <= 128; bn *= 2) {
@@ -1118,7 +1129,7 @@ I8Plan choose_plan(int M, int N, int K, bool gelu, int sms, int dev) {
     for (int ls = 0; ls <= 3 && (1 << ls) <= k_blocks && tiles <= cluster_room(ls, sms, dev); ++ls) {
       const int blocks = (k_blocks + (1 << ls) - 1) >> ls;
       consider(1.88 + (gelu ? 0.0175 : 0.012) * bn + (0.107 + 0.0005 * bn) * blocks + (ls ? 0.57 + 0.0035 * bn * ls : 0),
-               {false, bn, ls});
+               {BBH_I8_SPLIT, bn, 1 << ls});
     }
   }
   return best;
@@ -1161,32 +1172,45 @@ int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   I8Maps maps;
   cudaError_t e;
-  const bool few = few_is_faster(M, N, K, sms);
-  const I8Plan plan = few ? I8Plan{} : choose_plan(M, N, K, g, sms, dev);
-  if (few) {
-    e = launch_few_any(A, lda, W, ldw, p, bf16, g, sms, s);
-  } else if (!plan.pair) {
+  const I8Plan plan = choose_plan(M, N, K, g, sms, dev);
+  if (plan.kernel == BBH_I8_FEW) {
+    e = launch_few_any(A, lda, W, ldw, p, plan.tile, plan.part, bf16, g, s);
+  } else if (plan.kernel == BBH_I8_SPLIT) {
     maps.w = W;
     maps.ldw = ldw;
     rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, plan.bn, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, plan.tile, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return internal_fail(rc, "bbh_linear_i8: tensor map encoding failed");
-    switch (plan.bn) {
-      case 16: e = launch_small_bn<16>(maps, p, bf16, g, plan.log_splits, dev, s); break;
-      case 32: e = launch_small_bn<32>(maps, p, bf16, g, plan.log_splits, dev, s); break;
-      case 64: e = launch_small_bn<64>(maps, p, bf16, g, plan.log_splits, dev, s); break;
-      default: e = launch_small_bn<128>(maps, p, bf16, g, plan.log_splits, dev, s); break;
+    switch (plan.tile) {
+      case 16: e = launch_small_bn<16>(maps, p, bf16, g, plan.part, dev, s); break;
+      case 32: e = launch_small_bn<32>(maps, p, bf16, g, plan.part, dev, s); break;
+      case 64: e = launch_small_bn<64>(maps, p, bf16, g, plan.part, dev, s); break;
+      default: e = launch_small_bn<128>(maps, p, bf16, g, plan.part, dev, s); break;
     }
   } else {
     rc = encode_2d_bytes(&maps.A, A, M, K, lda, 1, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (!rc) rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, plan.bn / 2, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = encode_2d_bytes(&maps.W, W, N, K, ldw, 1, kBK, plan.tile / 2, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc)
       rc = tma_c ? encode_2d_bytes(&maps.C, C, M, N, ldc, 2, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B)
                  : (maps.C = maps.A, BBH_OK);
     if (rc) return internal_fail(rc, "bbh_linear_i8: tensor map encoding failed");
-    e = launch_pair_any(maps, p, plan.bn, bf16, g, tma_c, dev, sms, s);
+    e = launch_pair_any(maps, p, plan.tile, plan.part, bf16, g, tma_c, dev, sms, s);
   }
   if (e != cudaSuccess) return internal_fail(BBH_ERR_CUDA, std::string("bbh_linear_i8: ") + cudaGetErrorString(e));
+  return BBH_OK;
+}
+
+int bbh_linear_i8_plan(int M, int N, int K, int gelu, int* plan) {
+  using namespace bbh;
+  if (M < 1 || N < 1 || K < 1 || K > BBH_LINEAR_I8_MAX_K || !plan)
+    return internal_fail(BBH_ERR_ARG, "bbh_linear_i8_plan: M and N must be >= 1, K in [1, 131071], plan not null");
+  int dev = 0, sms = 0;
+  const int rc = unit_device(&dev, &sms);
+  if (rc) return rc;
+  const I8Plan p = choose_plan(M, N, K, gelu != 0, sms, dev);
+  plan[0] = p.kernel;
+  plan[1] = p.tile;
+  plan[2] = p.part;
   return BBH_OK;
 }
 

@@ -229,6 +229,14 @@ BBH_API int bbh_dequantize_i8(const int8_t* q, int64_t ldq, const float* scale, 
 BBH_API int bbh_linear_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw,
                           const float* w_scale, const uint16_t* bias, uint16_t* C, int64_t ldc, int M, int N, int K,
                           int gelu, int dtype, void* stream);
+/* The kernel that bbh_linear_i8 runs for these sizes on the current device (the output does not depend on it, bit
+ * for bit): plan[0] BBH_I8_FEW (1 to 16 tokens; plan[1] tiles of 8 tokens, plan[2] steps of K in flight),
+ * BBH_I8_SPLIT (few rows; plan[1] tokens a tile, plan[2] CTAs that share K) or BBH_I8_PAIR (many rows; plan[1]
+ * columns a tile, plan[2] columns a warp of the epilogue). M and N >= 1. */
+#define BBH_I8_FEW 0
+#define BBH_I8_SPLIT 1
+#define BBH_I8_PAIR 2
+BBH_API int bbh_linear_i8_plan(int M, int N, int K, int gelu, int plan[3]);
 /* Synchronises the current device and returns the device error code of its bbh_linear_i8 calls
  * (0 = none, 1 = a wait inside a kernel ran out: that call's output is invalid); optionally
  * clears it. */
