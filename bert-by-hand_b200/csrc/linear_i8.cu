@@ -836,7 +836,7 @@ __global__ void __launch_bounds__(I8SmallCfg<BN>::THREADS, 1)
 // eight warps every eighth 64 bytes of K, loaded straight into the fragments of mma.sync m16n8k32 (the
 // order of k is free as long as both operands have the same, so a lane's 16 consecutive bytes are four
 // of its fragments' words), and the partial sums meet in shared memory. 1 x 4096 x 4096: 3.3 us = 5.1 TB/s
-// of weights (they fit in L2 when repeated), 1 x 8192 x 8192 8.2 us = 8.2 TB/s.
+// of weights when they are in L2, 4.8 = 3.5 TB/s when they come from HBM; 1 x 8192 x 2048 3.3 and 4.8.
 constexpr int kFewWarps = 8;
 
 __device__ __forceinline__ void mma_i8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -1050,8 +1050,10 @@ cudaError_t launch_few(const int8_t* A, int64_t lda, const int8_t* W, int64_t ld
 }
 
 // Steps in flight of the kernel for one to 16 tokens: as many as a warp has (512 bytes of K each), where the CTAs are
-// too few to keep memory busy otherwise. 1 x 4096 x 4096: 8 steps 3.3 us, 4 steps 4.0, 2 steps 4.7; 1 x 384 x
-// 384: 2.5, 1.9, 1.5; 1 x 16384 x 4096 (1,024 CTAs): 10.3, 9.8, 9.2.
+// too few to keep memory busy otherwise. One token, us with 2 / 4 / 8 steps and the weights in L2: 4096 x 4096 4.4 /
+// 4.0 / 3.3, 4096 x 1536 3.3 / 2.9 / 4.6, 384 x 384 1.6 / 2.3 / 3.5, 8192 x 2048 (512 CTAs) 3.3 / 4.3 / 7.6; in HBM
+// 5.9 / 5.3 / 4.8, 3.9 / 3.7 / 5.2, 2.1 / 3.1 / 5.0, 4.8 / 6.3 / 9.2. At the border, N = 32 SMs: 4700 x 3500 5.0 /
+// 4.7 / 3.9, 5000 x 3300 5.2 / 4.7 / 6.1.
 int few_steps(int M, int N, int K, int sms) {
   if (M > 8 || K <= 1024 || N > 32 * sms) return 2;
   return K <= 2048 ? 4 : 8;
@@ -1066,9 +1068,11 @@ cudaError_t launch_few_any(const int8_t* A, int64_t lda, const int8_t* W, int64_
 }
 
 // Whether that kernel takes less time than the tcgen05 one (us, few rows / tcgen05), with the weights in L2: 1 x 4096
-// x 4096 3.3 / 4.1; 1 x 2048 x 8192 4.7 / 4.4; 4 x 16384 x 4096 8.8 / 8.7; 8 x 4096 x 4096 3.6 / 4.0; 8 x 16384 x
-// 4096 9.5 / 7.3; 16 x 1536 x 384 2.3 / 2.3; 16 x 1024 x 1024 2.1 / 2.9; 16 x 1024 x 4096 3.8 / 3.3; 16 x 4096 x 4096
-// 5.6 / 4.0; and in HBM: 1 x 4096 x 4096 4.5 / 5.2; 1 x 8192 x 2048 4.5 / 5.0; 1 x 16384 x 4096 13.9 / 12.4.
+// x 4096 3.3 / 4.2; 1 x 2048 x 8192 4.7 / 4.4; 4 x 16384 x 4096 8.8 / 8.7; 8 x 4096 x 4096 3.6 / 4.1; 8 x 16384 x
+// 4096 9.3 / 7.3; 16 x 1536 x 384 2.3 / 2.3; 16 x 1024 x 1024 2.1 / 2.9; 16 x 1024 x 4096 3.8 / 3.3; 16 x 4096 x 4096
+// 5.6 / 4.0; and in HBM, where a model's weights are for single tokens, K = 4096 and N = 4096, 5120, 6144, 8192, 11008,
+// 16384: one token 4.7 / 5.2, 6.6 / 6.6, 7.0 / 7.0, 7.8 / 7.9, 12.1 / 9.8, 14.0 / 12.3; eight 5.3 / 5.2, 7.1 / 6.9,
+// 7.6 / 7.3, 8.4 / 8.1, 12.7 / 9.9, 14.6 / 12.5. So nothing is lost from 16 Mi weights on.
 bool few_is_faster(int M, int N, int K, int sms) {
   const int64_t weights = int64_t(N) * K;
   if (M <= 8) return weights <= (int64_t(16) << 20) && (K <= 4096 || N > 16 * sms);

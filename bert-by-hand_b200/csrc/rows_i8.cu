@@ -9,10 +9,13 @@
 // rstd cancels out of q (q = rint(v w * 127 / max|v w|), scale = max|v w| * rstd / 127), so the
 // sum of squares and the maximum are reduced together, with one exchange between the warps
 // of a row. All arithmetic is fp32; the only roundings are those of the outputs.
-// Bound: HBM bytes (x, residual, sum, y or q; each moved once). On a B200 whose copies reach 6.5 TB/s:
-// 8192 x 4096 bf16 with a residual rmsnorm 41.2 us = 6.5 TB/s, rmsnorm_i8 37.2 = 6.3; without rmsnorm 22.0 = 6.1,
-// rmsnorm_i8 20.4 = 4.9 (its arithmetic per byte is twice that with one); quantize_i8 16.9 = 6.0, dequantize_i8
-// 15.0 = 6.7; 20000 x 1023 fp16 rmsnorm 15.8 = 5.2.
+// Bound: HBM bytes (x, residual, sum, y or q; each moved once). On a B200 whose copies reach 6.5 TB/s, with tensors that
+// change from call to call (more of them than L2 holds): 8192 x 4096 bf16 with a residual rmsnorm 41.7 us = 6.4 TB/s,
+// rmsnorm_i8 37.4 = 6.3; without rmsnorm 22.1 = 6.1, rmsnorm_i8 22.0 = 4.6 (its arithmetic per byte is twice that with
+// one); quantize_i8 18.2 = 5.5, dequantize_i8 17.6 = 5.7. 20000 x 1023 fp16, rows of every alignment: rmsnorm 18.6 =
+// 4.4, rmsnorm_i8 23.9 = 2.6, quantize_i8 16.4 = 3.7 (kShifted below: the weight is realigned for every chunk of
+// every row, and q goes through shared memory). The comparisons of variants further down were made with one set of
+// tensors, which L2 holds in part: up to a quarter shorter.
 #include "common.cuh"
 #include "epilogue.cuh"
 #include "internal.h"
@@ -43,7 +46,10 @@ struct RowParams {  // 96 bytes: above, a launch takes the host 0.35 us longer
 static_assert(sizeof(RowParams) == 96, "kernel arguments");
 
 constexpr int kRowBlock = 128;  // threads of a block when a row takes fewer
-constexpr int kRowMaxBlock = 512;  // leaves 128 registers a thread (only 2-byte accesses at the widest spill some)
+// Leaves 128 registers a thread, 64 where row_kernel asks for two blocks an SM. Spilled: with 2-byte accesses from three
+// or four chunks a thread on 100 to 220 bytes, at eight 550 to 1,580; kShifted with four chunks, or with a residual and
+// eight, 4 to 48; nothing with aligned rows.
+constexpr int kRowMaxBlock = 512;
 
 template <bool BF16>
 __device__ __forceinline__ float2 unpack16(uint32_t w) {
