@@ -22,6 +22,7 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cfloat>
 #include <string>
 
@@ -935,19 +936,22 @@ __global__ void __launch_bounds__(32 * kFewWarps)
 // ======================================================================== host side
 namespace {
 
+// What is asked or set once per device, by whichever thread comes first (several may: all find the same).
+using OncePerDevice = std::atomic<int>[64];
+
 // Once per device and kernel: opt in to the kernel's shared memory.
 template <typename K>
-cudaError_t opt_in(K kern, int smem, bool (&done)[64], int dev) {
+cudaError_t opt_in(K kern, int smem, OncePerDevice& done, int dev) {
   if (done[dev]) return cudaSuccess;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) done[dev] = true;
+  if (e == cudaSuccess) done[dev] = 1;
   return e;
 }
 
 // Clusters of `size` CTAs that can run at once, asked once per device and kernel.
 template <typename K>
-int max_clusters(K kern, int size, int threads, int smem, int sms, int (&cache)[64], int dev) {
-  if (cache[dev]) return cache[dev];
+int max_clusters(K kern, int size, int threads, int smem, int sms, OncePerDevice& cache, int dev) {
+  if (const int known = cache[dev]) return known;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -964,7 +968,8 @@ int max_clusters(K kern, int size, int threads, int smem, int sms, int (&cache)[
     (void)cudaGetLastError();
     n = sms / size;
   }
-  return cache[dev] = n;
+  cache[dev] = n;
+  return n;
 }
 
 struct I8Maps {
@@ -976,11 +981,11 @@ struct I8Maps {
 template <int BN, int COLS, bool BF16, bool GELU, bool TMA_C>
 cudaError_t launch_pair_i8(const I8Maps& m, const I8Params& p, int dev, int sms, cudaStream_t s) {
   using Cfg = I8PairCfg<BN, COLS>;
-  static bool done[64] = {};
+  static OncePerDevice done;
   auto kern = linear_i8_pair_kernel<BN, COLS, BF16, GELU, TMA_C>;
   const cudaError_t e = opt_in(kern, Cfg::SMEM, done, dev);
   if (e != cudaSuccess) return e;
-  static int pairs_of[64] = {};
+  static OncePerDevice pairs_of;
   const int64_t tiles = (int64_t(p.M) + 255) / 256 * ((p.N - 1) / BN + 1);
   const int most = max_clusters(kern, 2, Cfg::THREADS, Cfg::SMEM, sms, pairs_of, dev);
   const int pairs = static_cast<int>(tiles < most ? tiles : most);
@@ -1019,7 +1024,7 @@ cudaError_t launch_pair_any(const I8Maps& m, const I8Params& p, int bn, int cols
 template <int BN, bool BF16, bool GELU>
 cudaError_t launch_small_i8(const I8Maps& m, const I8Params& p, int splits, int dev, cudaStream_t s) {
   using Cfg = I8SmallCfg<BN>;
-  static bool done[64] = {};
+  static OncePerDevice done;
   auto kern = linear_i8_small_kernel<BN, BF16, GELU>;
   const cudaError_t e = opt_in(kern, Cfg::SMEM, done, dev);
   if (e != cudaSuccess) return e;
@@ -1091,8 +1096,8 @@ struct I8Plan {
 // do not all hold a whole number of large clusters.
 int cluster_room(int log_splits, int sms, int dev) {
   using Cfg = I8SmallCfg<64>;
-  static bool done[64] = {};
-  static int room[4][64] = {};
+  static OncePerDevice done;
+  static OncePerDevice room[4];
   if (log_splits == 0) return sms;
   auto kern = linear_i8_small_kernel<64, false, false>;
   if (opt_in(kern, Cfg::SMEM, done, dev) != cudaSuccess) return sms >> log_splits;

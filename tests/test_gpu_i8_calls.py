@@ -67,3 +67,48 @@ def test_other_threads_run_while_a_launch_waits(name):
     gap = max(b - a for a, b in zip(inside, inside[1:]))
     assert longest > 0.5, "no launch had to wait"
     assert gap < 0.4 * longest, (gap, longest)
+
+
+_FIRST_CALLS = """
+import sys, threading
+sys.path[:0] = [{here!r}]
+import torch, bbh
+sizes = [(1, 96, 64), (12, 96, 64), (20, 200, 4096), (100, 200, 1024), (64, 384, 384), (3000, 384, 64), (3000, 1536, 64)]
+g = torch.Generator(device="cuda").manual_seed(3)
+args = []
+for m, n, k in sizes:
+    x, w = (torch.randn(r, k, generator=g, device="cuda").half() for r in (m, n))
+    args.append((x, w))
+torch.cuda.synchronize()
+start, got, errors = threading.Barrier(8), [None] * 8, []
+def run(i):
+    try:
+        stream = torch.cuda.Stream()
+        start.wait()
+        with torch.cuda.stream(stream):
+            got[i] = [bbh.linear_i8(*bbh.rmsnorm_i8(x), *bbh.quantize_i8(w), gelu=True) for x, w in args]
+        stream.synchronize()
+    except BaseException as e:
+        errors.append(e)
+threads = [threading.Thread(target=run, args=(i,)) for i in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not errors, errors
+want = [bbh.linear_i8(*bbh.rmsnorm_i8(x), *bbh.quantize_i8(w), gelu=True) for x, w in args]
+assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
+assert bbh.linear_i8_device_error() == 0
+print("same")
+"""
+
+
+def test_first_calls_of_eight_threads_at_once():
+    """Threads run next to one another in these calls, the very first of a process among them."""
+    import os
+    import subprocess
+    import sys
+
+    import bbh
+
+    code = _FIRST_CALLS.format(here=os.path.dirname(os.path.abspath(bbh.__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stdout + r.stderr
