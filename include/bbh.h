@@ -204,7 +204,8 @@ BBH_API int bbh_mean_pool_l2(const uint16_t* hidden, const int32_t* cu_seqlens, 
 /* v = x + residual (fp32, not rounded; residual may be NULL); y = v / sqrt(mean(v^2) + eps) *
  * weight (NULL: ones). sum (NULL, or with a residual) receives v rounded to dtype. y and sum
  * may each be x or residual itself (same pointer, same stride). D in [1, 32768]. The squares are
- * fp32 too: a row whose sum of squares is above 3.4e38 (bf16 reaches it) gives y = 0. */
+ * fp32 too: a row whose sum of squares is above 3.4e38 (bf16 reaches it) gives y = 0, and with eps = 0 one whose
+ * squares all vanish (no |v| above 1e-23, bf16 again) infinities, or NaN where v is 0. */
 BBH_API int bbh_rmsnorm(const uint16_t* x, int64_t ldx, const uint16_t* residual, int64_t ldr, const uint16_t* weight,
                         uint16_t* y, int64_t ldy, uint16_t* sum, int64_t lds, int M, int D, float eps, int dtype,
                         void* stream);
