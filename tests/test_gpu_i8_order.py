@@ -85,3 +85,25 @@ def test_layers_that_share_buffers(M):
         h = bbh.linear_i8(*a, w, t, gelu=i % 2 == 0)
         torch.cuda.synchronize()
     assert torch.equal(got, h)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M,D", [(1, 1), (3, 9), (40, 384), (1000, 1023), (2, 20000)])
+def test_one_tensor_as_x_and_residual(M, D, dtype):
+    """x + x, also with an output over both: the same bits as from two copies."""
+    import bbh
+
+    x = torch.randn(M, D, generator=gen("twice", M, D), device=DEV).to(dtype)
+    y, v = bbh.rmsnorm(x, residual=x.clone())
+    q, s, _ = bbh.rmsnorm_i8(x, residual=x.clone())
+    for outputs in ("none", "y", "sum"):
+        t = x.clone()
+        out = {"none": {}, "y": {"out": t}, "sum": {"sum_out": t}}[outputs]
+        a, b = bbh.rmsnorm(t, residual=t, **out)
+        assert torch.equal(a, y) and torch.equal(b, v)
+    t = x.clone()
+    a, b, c = bbh.rmsnorm_i8(t, residual=t, sum_out=t)
+    assert torch.equal(a, q) and torch.equal(b, s) and torch.equal(c, v)
+    t = x.clone()
+    with pytest.raises(bbh.BBHError, match="overlap"):
+        bbh.rmsnorm(t, residual=t, out=t, sum_out=t)
