@@ -132,7 +132,7 @@ __device__ __forceinline__ float abs_to_16(float x) {
 // output and reweighted to equal ripple): Phi(-a) is within 1.8e-7 of itself up to a = 4, 2e-6 up to 5.75;
 // beyond, the polynomial keeps falling until ex2 gives 0 (from a = 11.5 on); a ends at 16, because infinity times that
 // 0 would be NaN: +inf stays +inf, -inf gives 0, and only NaN gives NaN. With the roundings of the sum and of ex2
-// the output is within 1e-7 max(|x|, 1).
+// the output is within 2e-7 max(|x|, 1).
 // Why this degree: of normal x 0.009 % of the fp16 outputs are the other neighbour of the exact value, 0.018 %
 // with fp32's erf. Degree 7 (Phi within 5.8e-6) has 0.20 %, and a quantiser behind the layer then rounds ten times
 // as many of its integers the other way, each of which the next layer spreads over a row; degree 9 0.018 to

@@ -223,7 +223,7 @@ BBH_API int bbh_quantize_i8(const uint16_t* x, int64_t ldx, int8_t* q, int64_t l
 /* y = q * scale[row], rounded to dtype. */
 BBH_API int bbh_dequantize_i8(const int8_t* q, int64_t ldq, const float* scale, uint16_t* y, int64_t ldy, int M, int D,
                               int dtype, void* stream);
-/* C[M, N] = (A W^T) * a_scale[m] * w_scale[n] (+ bias[n]) (+ erf-GELU, within 1e-7 max(|x|, 1) of
+/* C[M, N] = (A W^T) * a_scale[m] * w_scale[n] (+ bias[n]) (+ erf-GELU, within 2e-7 max(|x|, 1) of
  * the exact form before the rounding, +inf at +inf and 0 at -inf), A [M, K] and W [N, K] (nn.Linear layout)
  * int8, exact int32 sums. A and W 16-byte aligned with row strides of whole 16 bytes, of whole 128 for
  * the best speed (K itself may be any value in [1, 131071]); C and bias (dtype, bias may be NULL) of any alignment and N. */
